@@ -4,13 +4,17 @@ conversions between 8-bit and wide states.
 
 The 8-bit form of a state: blocks of 128 consecutive elements of the flattened
 tensor, each with one fp32 scale s.
-  signed (first moments): s = max |x|,        code q = sgn(x) rint(127 sqrt(|x| / s)),   value s q |q| / 127^2
-  root (second moments):  s = max sqrt(x),    code q = rint(255 sqrt(sqrt(x) / s)) >= 1 where x > 0,
-                                              value (s (q / 255)^2)^2
+  signed (first moments): s = max |x|,      code q = sgn(x) floor(127 sqrt(|x| / s) + u),  value s q |q| / 127^2
+  root (second moments):  s = max sqrt(x),  code q = floor(255 sqrt(sqrt(x) / s) + u), at least 1 where x > 0,
+                                            value (s (q / 255)^2)^2
   pair (master weights):  bf16 weight p = bf16(w) and remainder bf16(w - p), value p + remainder
-Ties go to the even code. A block that holds a value that is not finite has
-the scale NaN; one that holds only zeros has the scale 0.
+u is 1/2 (nearest) in a conversion. In a step it runs evenly over [0, 1) from
+step to step, so that a change smaller than a code step is kept on average:
+with h = 2654435769 i + 1821285621 t (+ 2^31 for signed) modulo 2^32 for element
+i in step t, u = floor(h / 2^9) / 2^23. A block that holds a value that is not
+finite has the scale NaN; one that holds only zeros has the scale 0.
 """
+import ctypes
 import math
 import os
 import sys
@@ -169,24 +173,32 @@ def _blocks(x):
     return torch.nn.functional.pad(flat, (0, -flat.numel() % BLOCK)).view(-1, BLOCK)
 
 
-def _nearest(x, s, levels):
-    """rint(levels sqrt(x / s)): in 64 bits, so that the side of a border does not hang on a rounding."""
-    return (levels * (x.double() / torch.where(s > 0, s, 1.0).double()[:, None]).sqrt()).round()
+def _dither(b, t, phase):
+    if t is None:
+        return 0.5
+    i = torch.arange(b.numel(), device=b.device).view(b.shape)
+    return ((i * 2654435769 + t * 1821285621 + phase) % 2 ** 32 // 2 ** 9).double() / 2 ** 23
 
 
-def _write_signed(x):
+def _code(x, s, levels, u):
+    """floor(levels sqrt(x / s) + u): in 64 bits, so that the side of a border does not hang on a rounding."""
+    y = levels * (x.double() / torch.where(s > 0, s, 1.0).double()[:, None]).sqrt()
+    return torch.where((s > 0)[:, None], (y + u).floor().clamp(max=levels), 0.0)
+
+
+def _write_signed(x, t=None):
     b = _blocks(x.float())
     s = b.abs().amax(1)
     s = torch.where(s.isfinite(), torch.where(s >= 2.0 ** -126, s, 0.0), math.nan)
-    q = torch.where((s > 0)[:, None], _nearest(b.abs(), s, 127) * b.sign(), 0.0)
+    q = _code(b.abs(), s, 127, _dither(b, t, 2 ** 31)) * b.sign()
     return q.to(torch.int8).view(-1)[: x.numel()].view(x.shape), s
 
 
-def _write_root(x):
+def _write_root(x, t=None):
     b = _blocks(x.float())
     s = b.amax(1).sqrt()
     s = torch.where(s.isfinite(), s, math.nan)
-    q = torch.where((s > 0)[:, None], torch.where(b > 0, _nearest(b.sqrt(), s, 255).clamp(min=1), 0.0), 0.0)
+    q = torch.maximum(_code(b.sqrt(), s, 255, _dither(b, t, 0)), ((b > 0) & (s > 0)[:, None]).double())
     return q.to(torch.uint8).view(-1)[: x.numel()].view(x.shape), s
 
 
@@ -212,8 +224,8 @@ def _plain_adamw(case, one, t):
         w = w - LR * wd * w
     w = w - LR / (1 - BETA1 ** t) * m / (v.sqrt() / math.sqrt(1 - b2 ** t) + EPS)
     p = one["p"].copy_(w)
-    one["m"], one["ms"] = _write_signed(m)
-    one["v"], one["vs"] = _write_root(v)
+    one["m"], one["ms"] = _write_signed(m, t)
+    one["v"], one["vs"] = _write_root(v, t)
     out = {"p": p, "exp_avg": _read_signed(one["m"], one["ms"]).bfloat16(),
            "exp_avg_sq": _read_root(one["v"], one["vs"]).bfloat16()}
     if one["rem"] is not None:
@@ -224,16 +236,16 @@ def _plain_adamw(case, one, t):
     return out
 
 
-def _plain_momentum(case, one):
+def _plain_momentum(case, one, t):
     shape = one["g"].shape
-    many = [_plain_matrix(case, one["g"][i].float(), one["m"][i], one["ms"][i]) for i in range(shape[0])]
+    many = [_plain_matrix(case, one["g"][i].float(), one["m"][i], one["ms"][i], t) for i in range(shape[0])]
     u, sq, m, ms, val = (torch.stack(x) for x in zip(*many))
     one["m"], one["ms"] = m, ms
     return {"u": u, "squares": sq, "momentum": val}
 
 
-def _plain_matrix(case, g, q, s):
-    m, s = _write_signed(MOMENTUM * _read_signed(q, s) + (1 - MOMENTUM) * g)
+def _plain_matrix(case, g, q, s, t):
+    m, s = _write_signed(MOMENTUM * _read_signed(q, s) + (1 - MOMENTUM) * g, t)
     val = _read_signed(m, s)
     u = (MOMENTUM * val + (1 - MOMENTUM) * g if case["nesterov"] else val).bfloat16()
     sq = u.float().square().view(-1)
@@ -260,7 +272,7 @@ def run(s):
     if case["op"] == "adamw":
         return [_plain_adamw(case, one, s["t"]) for one in s["items"]]
     if case["op"] == "momentum":
-        return [_plain_momentum(case, one) for one in s["items"]]
+        return [_plain_momentum(case, one, s["t"]) for one in s["items"]]
     if case["op"] == "encode":
         return [_plain_encode(one) for one in s["items"]]
     return [_plain_decode(case, one) for one in s["items"]]
@@ -300,7 +312,7 @@ def _handles(case, s):
     elif case["op"] == "momentum":
         from sol_b200 import _lib
         lib, keep = _lib.load(), []
-        arr, scales = (_lib.NormuonBatch * len(s["items"]))(), []
+        arr, scales, steps = (_lib.NormuonBatch * len(s["items"]))(), [], []
         for i, one in enumerate(s["items"]):
             S, r, c = one["g"].shape
             one["u"] = torch.empty(S, r, c, dtype=torch.bfloat16, device="cuda")
@@ -311,9 +323,11 @@ def _handles(case, s):
             sc = _lib.ptr_array([x.data_ptr() for x in one["ms"]])
             keep += [grads, bufs, sc]
             scales.append(_lib.addr(sc))
+            steps.append((ctypes.c_uint32 * S)())
             arr[i] = _lib.NormuonBatch(S=S, r=r, c=c, grads=_lib.addr(grads), bufs=_lib.addr(bufs),
                                        u=one["u"].data_ptr(), partial=one["sq"].data_ptr())
-        s["call"] = (arr, _lib.ptr_array(scales), len(s["items"]), _lib.dtype_code(_dtype(case)), MOMENTUM,
+        s["steps"] = steps
+        s["call"] = (arr, _lib.ptr_array(scales), _lib.ptr_array([_lib.addr(x) for x in steps]), len(s["items"]), _lib.dtype_code(_dtype(case)), MOMENTUM,
                      int(case["nesterov"]), None)
         s["keep"] = keep
 
@@ -333,6 +347,9 @@ def _own(s):
     from sol_b200 import state8
     if case["op"] == "momentum":
         from sol_b200 import _lib
+        s["t"] += 1
+        for x in s["steps"]:
+            x[:] = [s["t"]] * len(x)
         _lib.check(_lib.load().b2o_normuon_front8_multi(*s["call"], _lib.stream_ptr()), "normuon_front8")
         state8.decode([(q, sc, "signed") for one in items for q, sc in zip(one["m"], one["ms"])],
                       out=[x for one in items for x in one["val"]])
@@ -350,7 +367,7 @@ def _own(s):
 
 
 # -------------------------------------------------------- 64-bit results ---
-def _coded(x, root):
+def _coded(x, root, step=None):
     """The value that the 8-bit code of each element stands for, from the definition, in 64 bits."""
     n, levels = x.numel(), 255.0 if root else 127.0
     size = x.abs().sqrt() if root else x.abs()
@@ -358,7 +375,11 @@ def _coded(x, root):
     rows[:n] = size.reshape(-1)
     rows = rows.view(-1, BLOCK)
     top = rows.max(dim=1, keepdim=True).values.float().double()  # scales are kept in 32 bits
-    q = torch.round(levels * torch.sqrt(torch.nan_to_num(rows / top)))
+    part = torch.full_like(rows, 0.5)
+    if step is not None:
+        turn = torch.arange(rows.numel(), device=x.device).mul_(0x9E3779B9).add_((0x6C8E9CF5 * step + (0 if root else 1 << 31)) & 0xFFFFFFFF)
+        part = ((turn & 0xFFFFFFFF) >> 9).view(rows.shape).double().mul_(2.0 ** -23)
+    q = torch.floor(levels * torch.sqrt(torch.nan_to_num(rows / top)) + part).clamp_(max=levels)
     if root:
         q = torch.maximum(q, (rows > 0).double())
     size = (top * (q / levels) ** 2).view(-1)[:n].view(x.shape)
@@ -391,7 +412,7 @@ def exact(case, seed):
                 w = w * (1 - shrink)
             root = (v / (1 - b2 ** t)).sqrt()
             w = w - LR * (m / (1 - BETA1 ** t)) / (root + EPS)
-            d = {"p": w, "exp_avg": _coded(m, False)[0], "exp_avg_sq": _coded(v, True)[0]}
+            d = {"p": w, "exp_avg": _coded(m, False, t)[0], "exp_avg_sq": _coded(v, True, t)[0]}
             if one["rem"] is not None:
                 d["master"] = w
             if one["ema"] is not None:
@@ -399,7 +420,7 @@ def exact(case, seed):
         elif case["op"] == "momentum":
             d = {"u": [], "squares": [], "momentum": []}
             for g, q, sc in zip(one["g"].double(), one["m"], one["ms"]):
-                val = _coded(MOMENTUM * _stands_for(q, sc, False) + (1 - MOMENTUM) * g, False)[0]
+                val = _coded(MOMENTUM * _stands_for(q, sc, False) + (1 - MOMENTUM) * g, False, STEP + 1)[0]
                 u = MOMENTUM * val + (1 - MOMENTUM) * g if case["nesterov"] else val
                 d["u"].append(u)
                 parts = u.to(torch.bfloat16).double().square().flatten().split(PART)
