@@ -10,7 +10,7 @@ tensor, each with one fp32 scale s.
   pair (master weights):  bf16 weight p = bf16(w) and remainder bf16(w - p), value p + remainder
 u is 1/2 (nearest) in a conversion. In a step it runs evenly over [0, 1) from
 step to step, so that a change smaller than a code step is kept on average:
-with h = 2654435769 i + 1821285621 t (+ 2^31 for signed) modulo 2^32 for element
+with h = 2654435769 i + 1779033703 t (+ 2^31 for signed) modulo 2^32 for element
 i in step t, u = floor(h / 2^9) / 2^23. A block that holds a value that is not
 finite has the scale NaN; one that holds only zeros has the scale 0.
 """
@@ -177,7 +177,7 @@ def _dither(b, t, phase):
     if t is None:
         return 0.5
     i = torch.arange(b.numel(), device=b.device).view(b.shape)
-    return ((i * 2654435769 + t * 1821285621 + phase) % 2 ** 32 // 2 ** 9).double() / 2 ** 23
+    return ((i * 2654435769 + t * 1779033703 + phase) % 2 ** 32 // 2 ** 9).double() / 2 ** 23
 
 
 def _code(x, s, levels, u):
@@ -377,7 +377,7 @@ def _coded(x, root, step=None):
     top = rows.max(dim=1, keepdim=True).values.float().double()  # scales are kept in 32 bits
     part = torch.full_like(rows, 0.5)
     if step is not None:
-        turn = torch.arange(rows.numel(), device=x.device).mul_(0x9E3779B9).add_((0x6C8E9CF5 * step + (0 if root else 1 << 31)) & 0xFFFFFFFF)
+        turn = torch.arange(rows.numel(), device=x.device).mul_(0x9E3779B9).add_((0x6A09E667 * step + (0 if root else 1 << 31)) & 0xFFFFFFFF)
         part = ((turn & 0xFFFFFFFF) >> 9).view(rows.shape).double().mul_(2.0 ** -23)
     q = torch.floor(levels * torch.sqrt(torch.nan_to_num(rows / top)) + part).clamp_(max=levels)
     if root:
