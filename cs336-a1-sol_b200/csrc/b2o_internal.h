@@ -16,6 +16,13 @@ int num_sms();
 // ---- streaming.cu
 int adamw_step(const b2o_adamw_tensor* tensors, int ntensors, const b2o_adamw_group* groups,
                int ngroups, int param_dtype, int state_dtype, float ema_weight, cudaStream_t stream);
+// ---- state8.cu
+int64_t state_blocks(int64_t numel);
+int state_encode(const b2o_state_tensor* tensors, int ntensors, cudaStream_t stream);
+int state_decode(const b2o_state_tensor* tensors, int ntensors, cudaStream_t stream);
+int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8_group* groups, int ngroups,
+                int param_dtype, float ema_weight, cudaStream_t stream);
+// ---- streaming.cu (continued)
 int ema_update(float* const* shadows, const void* const* params, const int64_t* numels, int nt,
                int param_dtype, float w, cudaStream_t stream);
 int ema_copy_to_params(const float* const* shadows, void* const* params, const int64_t* numels, int nt,
@@ -32,6 +39,11 @@ int normuon_front_multi(const b2o_normuon_batch* batches, int nb, int dtype, flo
                         int nesterov, const float* grad_scale, cudaStream_t stream);
 int normuon_prescale(const b2o_normuon_batch* batches, int nb, int dtype, float w_small, float w_large,
                      int nesterov, const float* grad_scale, float norm_eps, float norm_safety, cudaStream_t stream);
+int normuon_front8_multi(const b2o_normuon_batch* batches, float* const* const* buf_scales,
+                         const uint32_t* const* buf_steps, int nb, int dtype, double beta, int nesterov,
+                         const float* grad_scale, cudaStream_t stream);
+int normuon_prescale8(const b2o_normuon_batch* batches, float* const* const* buf_scales, int nb, int dtype, double beta,
+                      int nesterov, const float* grad_scale, float norm_eps, float norm_safety, cudaStream_t stream);
 // ---- clip.cu
 int64_t clip_scratch_floats(const int64_t* numels, int n);
 int clip_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int n, float max_norm,

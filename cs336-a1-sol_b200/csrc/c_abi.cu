@@ -128,6 +128,21 @@ int b2o_adamw_step(const b2o_adamw_tensor* tensors, int ntensors, const b2o_adam
                     static_cast<cudaStream_t>(stream));
 }
 
+int64_t b2o_state_blocks(int64_t numel) { return state_blocks(numel); }
+
+int b2o_state_encode(const b2o_state_tensor* tensors, int ntensors, void* stream) {
+  return state_encode(tensors, ntensors, static_cast<cudaStream_t>(stream));
+}
+
+int b2o_state_decode(const b2o_state_tensor* tensors, int ntensors, void* stream) {
+  return state_decode(tensors, ntensors, static_cast<cudaStream_t>(stream));
+}
+
+int b2o_adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8_group* groups, int ngroups,
+                    int param_dtype, float ema_weight, void* stream) {
+  return adamw8_step(tensors, ntensors, groups, ngroups, param_dtype, ema_weight, static_cast<cudaStream_t>(stream));
+}
+
 int b2o_ema_update(float* const* shadows, const void* const* params, const int64_t* numels, int ntensors,
                    int param_dtype, float weight, void* stream) {
   return ema_update(shadows, params, numels, ntensors, param_dtype, weight, static_cast<cudaStream_t>(stream));
@@ -200,6 +215,20 @@ int b2o_normuon_prescale(const b2o_normuon_batch* batches, int nbatches, int dty
                          int nesterov, const float* d_grad_scale, float norm_eps, float norm_safety, void* stream) {
   return normuon_prescale(batches, nbatches, dtype, w_small, w_large, nesterov, d_grad_scale, norm_eps, norm_safety,
                           static_cast<cudaStream_t>(stream));
+}
+
+int b2o_normuon_front8_multi(const b2o_normuon_batch* batches, float* const* const* buf_scales,
+                             const uint32_t* const* buf_steps, int nbatches, int dtype, double beta, int nesterov,
+                             const float* d_grad_scale, void* stream) {
+  return normuon_front8_multi(batches, buf_scales, buf_steps, nbatches, dtype, beta, nesterov, d_grad_scale,
+                              static_cast<cudaStream_t>(stream));
+}
+
+int b2o_normuon_prescale8(const b2o_normuon_batch* batches, float* const* const* buf_scales, int nbatches, int dtype,
+                          double beta, int nesterov, const float* d_grad_scale, float norm_eps, float norm_safety,
+                          void* stream) {
+  return normuon_prescale8(batches, buf_scales, nbatches, dtype, beta, nesterov, d_grad_scale, norm_eps, norm_safety,
+                           static_cast<cudaStream_t>(stream));
 }
 
 int64_t b2o_clip_scratch_floats(const int64_t* numels, int n) { return clip_scratch_floats(numels, n); }

@@ -1,13 +1,15 @@
 // HBM-bound streaming kernels of the optimizer step (sm_100a):
 //   * fused AdamW (+ EMA)                 torch.optim.AdamW(fused=True), sol_modules.py:468-476
 //   * stand-alone EMA and EMA->param copy EmaWeights.update/averaged, sol_modules.py:1255-1280
-//   * NorMuon front (momentum, Nesterov)  sol_modules.py:390-394
+//   * NorMuon front (momentum, Nesterov)  sol_modules.py:390-394, also with an 8-bit momentum
 //   * NorMuon finish + apply              sol_modules.py:396-424
 // All kernels move 16-byte vectors, size their grids in multiples of the SM
 // count and take tensor lists by value as kernel parameters (no host->device
 // copies of pointer tables).
 #include "b2o_common.cuh"
 #include "b2o_internal.h"
+#include "state8.cuh"
+#include "vec_io.cuh"
 
 #include <algorithm>
 #include <cstdio>
@@ -16,49 +18,6 @@
 #include <vector>
 
 namespace b2o {
-
-// ------------------------------------------------------------ vector I/O ---
-struct alignas(16) U16x8 { uint16_t v[8]; };
-struct alignas(16) F32x4 { float v[4]; };
-
-template <typename T> struct Elem;
-template <> struct Elem<float> {
-  __device__ static void load8(const float* p, float* o) {
-    F32x4 a = *reinterpret_cast<const F32x4*>(p);
-    F32x4 b = *reinterpret_cast<const F32x4*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { o[i] = a.v[i]; o[4 + i] = b.v[i]; }
-  }
-  __device__ static void store8(float* p, const float* x) {
-    F32x4 a, b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { a.v[i] = x[i]; b.v[i] = x[4 + i]; }
-    *reinterpret_cast<F32x4*>(p) = a;
-    *reinterpret_cast<F32x4*>(p + 4) = b;
-  }
-  __device__ static float load1(const float* p) { return *p; }
-  __device__ static void store1(float* p, float x) { *p = x; }
-  // value after rounding to the storage type
-  __device__ static float rnd(float x) { return x; }
-};
-template <> struct Elem<uint16_t> {  // bf16 stored as raw bits
-  __device__ static void load8(const uint16_t* p, float* o) {
-    U16x8 a = *reinterpret_cast<const U16x8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = bf16_to_f32(a.v[i]);
-  }
-  __device__ static void store8(uint16_t* p, const float* x) {
-    U16x8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a.v[i] = f32_to_bf16(x[i]);
-    *reinterpret_cast<U16x8*>(p) = a;
-  }
-  __device__ static float load1(const uint16_t* p) { return bf16_to_f32(*p); }
-  __device__ static void store1(uint16_t* p, float x) { *p = f32_to_bf16(x); }
-  __device__ static float rnd(float x) { return round_bf16(x); }
-};
-
-static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ================================================================ AdamW ===
 constexpr int kAdamMaxTensors = 96;
@@ -593,14 +552,11 @@ static int fill_header(const b2o_normuon_batch* batches, int nb, const char* wha
   return 0;
 }
 
-// repair = false: the front pass; true: the prescale pass that follows it
-// (same batches and arguments).
-static int front_launch(const b2o_normuon_batch* batches, int nb, int dtype, float w_small, float w_large,
-                        int nesterov, const float* grad_scale, bool repair, float norm_eps, float norm_safety,
-                        cudaStream_t stream) {
-  if (dtype != B2O_F32 && dtype != B2O_BF16) { set_error("normuon_front: bad dtype"); return -1; }
-  FrontTable tab;
-  int nmats = 0, ncta = 0;
+// The gradient, momentum and output pointers of a front or prescale call.
+// buf_align: what a vector access of the momentum must be aligned to, in bytes.
+template <typename Table>
+static int fill_front(const b2o_normuon_batch* batches, int nb, const float* grad_scale, int buf_align, Table& tab,
+                      int& nmats, int& ncta) {
   if (int e = fill_header(batches, nb, "normuon_front", normuon_front_parts, tab.h, nmats, ncta)) return e;
   memset(tab.g, 0, sizeof(tab.g));
   memset(tab.buf, 0, sizeof(tab.buf));
@@ -614,7 +570,7 @@ static int front_launch(const b2o_normuon_batch* batches, int nb, int dtype, flo
       if (!b.grads[s] || !b.bufs[s]) { set_error("normuon_front: null matrix pointer"); return -1; }
       tab.g[bi.mat0 + s] = b.grads[s];
       tab.buf[bi.mat0 + s] = b.bufs[s];
-      vec_ok = vec_ok && aligned16(b.grads[s]) && aligned16(b.bufs[s]);
+      vec_ok = vec_ok && aligned16(b.grads[s]) && (reinterpret_cast<uintptr_t>(b.bufs[s]) & (buf_align - 1)) == 0;
     }
     bi.vec_ok = vec_ok;
     bi.u = b.u;
@@ -627,12 +583,29 @@ static int front_launch(const b2o_normuon_batch* batches, int nb, int dtype, flo
       set_error("normuon_front: x0_half needs prescale, xscale and flags"); return -1;
     }
   }
+  return 0;
+}
+
+// this step's scales, next step's k, flags
+static int prescale_launch(const MultiHeader& h, int nmats, float norm_eps, float norm_safety, cudaStream_t stream) {
+  launch_pdl(normuon_prescale_kernel, dim3((nmats * 32 + 127) / 128), dim3(128), 0, stream, h, nmats, norm_eps,
+             norm_safety);
+  count_launch();
+  return check_launch("normuon_prescale");
+}
+
+// repair = false: the front pass; true: the prescale pass that follows it
+// (same batches and arguments).
+static int front_launch(const b2o_normuon_batch* batches, int nb, int dtype, float w_small, float w_large,
+                        int nesterov, const float* grad_scale, bool repair, float norm_eps, float norm_safety,
+                        cudaStream_t stream) {
+  if (dtype != B2O_F32 && dtype != B2O_BF16) { set_error("normuon_front: bad dtype"); return -1; }
+  FrontTable tab;
+  int nmats = 0, ncta = 0;
+  if (int e = fill_front(batches, nb, grad_scale, 16, tab, nmats, ncta)) return e;
   if (repair) {
-    // this step's scales, next step's k, flags; then X0 of the flagged matrices
-    launch_pdl(normuon_prescale_kernel, dim3((nmats * 32 + 127) / 128), dim3(128), 0, stream, tab.h, nmats,
-               norm_eps, norm_safety);
-    count_launch();
-    if (int e = check_launch("normuon_prescale")) return e;
+    // then X0 of the flagged matrices
+    if (int e = prescale_launch(tab.h, nmats, norm_eps, norm_safety, stream)) return e;
     const int rgrid = nmats * kRepairCtas;
     if (dtype == B2O_F32)
       launch_pdl(normuon_x0_repair_kernel<float>, dim3(rgrid), dim3(kFrontThreads), 0, stream, tab, w_small,
@@ -672,6 +645,171 @@ int normuon_front(const void* const* grads, void* const* bufs, int S, int r, int
   b.S = S; b.r = r; b.c = c;
   b.grads = grads; b.bufs = bufs; b.u = U; b.partial = partial;
   return normuon_front_multi(&b, 1, dtype, w_small, w_large, nesterov, nullptr, stream);
+}
+
+// ============================================ NorMuon front, 8-bit momentum ===
+// The front pass with the momentum in 8 bits (state8.cuh): 6.06 bytes an
+// element for bf16 gradients (gradient 2, code 1 + 1, u 2, scales) against 8
+// with a bf16 momentum. m = beta m + (1 - beta) g is rounded to its code in
+// registers (a block's largest magnitude over 16 lanes), and u is taken from
+// the value that the code stands for: the repair pass, which has only the
+// stored momentum, then rewrites X0 exactly.
+struct Front8Table {
+  MultiHeader h;
+  const void* g[kMaxMultiMats];
+  void* buf[kMaxMultiMats];     // int8 codes
+  float* scale[kMaxMultiMats];  // one per 128 elements
+  uint32_t step[kMaxMultiMats];  // the step count that the codes' offsets run with
+  const float* gscale;
+};
+
+template <typename T, bool REPAIR>
+__device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, float beta, float w1, int nesterov) {
+  const MultiBatchInfo& bi = tab.h.b[find_batch_cta(tab.h, cta)];
+  const int local = cta - bi.cta0;
+  const int s = local / bi.nparts;
+  const int part = local - s * bi.nparts;
+  const int64_t rc = bi.rc;
+  const T* G = static_cast<const T*>(tab.g[bi.mat0 + s]);
+  void* B = tab.buf[bi.mat0 + s];
+  float* SC = tab.scale[bi.mat0 + s];
+  const uint32_t step = tab.step[bi.mat0 + s];
+  uint16_t* Us = bi.u + static_cast<int64_t>(s) * rc;
+  const bool x0 = bi.x0_half != 0;
+  const float kx = x0 ? bi.prescale[s] : 1.0f;
+  const int64_t base = static_cast<int64_t>(part) * kFrontPart;
+  const int64_t end = min(rc, base + kFrontPart);
+  const bool clip = tab.gscale != nullptr;
+  const float gs = clip ? *tab.gscale : 1.0f;
+  const int lane = threadIdx.x & 31;
+  float pacc = 0.f;
+  for (int64_t tile = base + (threadIdx.x >> 5) * kQ8Tile; tile < end; tile += (kFrontThreads / 32) * kQ8Tile) {
+    const int64_t i = tile + lane * 8;
+    const bool vec = bi.vec_ok && i + 8 <= end;
+    float g[8], m[8];
+    if (vec) {
+      Elem<T>::load8(G + i, g);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = i + k < end ? Elem<T>::load1(G + i + k) : 0.0f;
+    }
+    if (clip) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = Elem<T>::rnd(g[k] * gs);
+    }
+    const float sc = i < end ? SC[i / kQ8Block] : 0.0f;
+    uint2 codes = load_codes(B, i, end, vec);
+    unpack_signed(codes, sc, m);
+    if (!REPAIR) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m[k] = __fadd_rn(__fmul_rn(beta, m[k]), __fmul_rn(w1, g[k]));
+      const BlockScale b = signed_scale(block_max(max_abs_bits(m)));
+      codes = pack_signed<true>(m, b, dither_of(i, step));
+      if (i < end) {
+        store_codes(B, i, end, vec, codes);
+        if ((lane & 15) == 0) SC[i / kQ8Block] = b.s;
+      }
+      unpack_signed(codes, b.s, m);
+    }
+    float u[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      u[k] = round_bf16(nesterov ? __fadd_rn(__fmul_rn(beta, m[k]), __fmul_rn(w1, g[k])) : m[k]);
+      if (i + k < end) pacc = fmaf(u[k], u[k], pacc);
+    }
+    if (vec) {
+      store_u8(Us + i, u, x0, kx);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + k < end) Us[i + k] = x0 ? f32_to_f16(u[k] * kx) : f32_to_bf16(u[k]);
+    }
+  }
+  if (REPAIR) return;
+  // fixed-order block reduction of this part
+  __shared__ float red[kFrontThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) pacc += __shfl_xor_sync(0xffffffffu, pacc, o);
+  if (lane == 0) red[threadIdx.x >> 5] = pacc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.f;
+    for (int q = 0; q < kFrontThreads / 32; ++q) t += red[q];
+    bi.partial[static_cast<int64_t>(s) * bi.nparts + part] = t;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFrontThreads) normuon_front8_kernel(const __grid_constant__ Front8Table tab,
+                                                                       float beta, float w1, int nesterov) {
+  pdl_wait();
+  front8_body<T, false>(tab, blockIdx.x, beta, w1, nesterov);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFrontThreads) normuon_x0_repair8_kernel(const __grid_constant__ Front8Table tab,
+                                                                           float beta, float w1, int nesterov) {
+  pdl_wait();
+  const int m = blockIdx.x / kRepairCtas;
+  const int sub = blockIdx.x - m * kRepairCtas;
+  int kb = 0;
+  while (kb + 1 < tab.h.nb && m >= tab.h.b[kb + 1].mat0) ++kb;
+  const MultiBatchInfo& bi = tab.h.b[kb];
+  const int s = m - bi.mat0;
+  if (!bi.x0_half || !bi.flags[s]) return;
+  for (int part = sub; part < bi.nparts; part += kRepairCtas)
+    front8_body<T, true>(tab, bi.cta0 + s * bi.nparts + part, beta, w1, nesterov);
+}
+
+static int front8_launch(const b2o_normuon_batch* batches, float* const* const* buf_scales,
+                         const uint32_t* const* buf_steps, int nb, int dtype, double beta, int nesterov, const float* grad_scale, bool repair, float norm_eps,
+                         float norm_safety, cudaStream_t stream) {
+  if (dtype != B2O_F32 && dtype != B2O_BF16) { set_error("normuon_front8: bad dtype"); return -1; }
+  if (!(beta >= 0.0 && beta < 1.0)) { set_error("normuon_front8: momentum must be in [0, 1)"); return -1; }
+  if (!buf_scales || (!buf_steps && !repair)) { set_error("normuon_front8: no scales or steps"); return -1; }
+  Front8Table tab;
+  int nmats = 0, ncta = 0;
+  if (int e = fill_front(batches, nb, grad_scale, 8, tab, nmats, ncta)) return e;
+  memset(tab.scale, 0, sizeof(tab.scale));
+  memset(tab.step, 0, sizeof(tab.step));
+  for (int k = 0; k < nb; ++k) {
+    for (int s = 0; s < batches[k].S; ++s) {
+      if (!buf_scales[k] || !buf_scales[k][s]) { set_error("normuon_front8: null scale pointer"); return -1; }
+      tab.scale[tab.h.b[k].mat0 + s] = buf_scales[k][s];
+      if (!repair && !buf_steps[k]) { set_error("normuon_front8: null step list"); return -1; }
+      if (!repair) tab.step[tab.h.b[k].mat0 + s] = buf_steps[k][s];
+    }
+  }
+  const float b = static_cast<float>(beta), w1 = static_cast<float>(1.0 - beta);
+  if (repair) {
+    if (int e = prescale_launch(tab.h, nmats, norm_eps, norm_safety, stream)) return e;
+    const int rgrid = nmats * kRepairCtas;
+    if (dtype == B2O_F32)
+      launch_pdl(normuon_x0_repair8_kernel<float>, dim3(rgrid), dim3(kFrontThreads), 0, stream, tab, b, w1, nesterov);
+    else
+      launch_pdl(normuon_x0_repair8_kernel<uint16_t>, dim3(rgrid), dim3(kFrontThreads), 0, stream, tab, b, w1,
+                 nesterov);
+    count_launch();
+    return check_launch("normuon_x0_repair8");
+  }
+  if (dtype == B2O_F32)
+    launch_pdl(normuon_front8_kernel<float>, dim3(ncta), dim3(kFrontThreads), 0, stream, tab, b, w1, nesterov);
+  else
+    launch_pdl(normuon_front8_kernel<uint16_t>, dim3(ncta), dim3(kFrontThreads), 0, stream, tab, b, w1, nesterov);
+  count_launch();
+  return check_launch("normuon_front8");
+}
+
+int normuon_front8_multi(const b2o_normuon_batch* batches, float* const* const* buf_scales,
+                         const uint32_t* const* buf_steps, int nb, int dtype, double beta, int nesterov,
+                         const float* grad_scale, cudaStream_t stream) {
+  return front8_launch(batches, buf_scales, buf_steps, nb, dtype, beta, nesterov, grad_scale, false, 0.f, 1.f, stream);
+}
+
+int normuon_prescale8(const b2o_normuon_batch* batches, float* const* const* buf_scales, int nb, int dtype, double beta,
+                      int nesterov, const float* grad_scale, float norm_eps, float norm_safety, cudaStream_t stream) {
+  return front8_launch(batches, buf_scales, nullptr, nb, dtype, beta, nesterov, grad_scale, true, norm_eps,
+                       norm_safety, stream);
 }
 
 // ====================================================== NorMuon finish ===

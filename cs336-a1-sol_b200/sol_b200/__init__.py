@@ -2,16 +2,18 @@
 
 Public surface (names of transformer_lm.sol_modules):
   build_optimizers, NorMuonGNS, EmaWeights, plus AdamW (the fused AdamW that
-  build_optimizers returns). ``install()`` points transformer_lm.sol_modules at
+  build_optimizers returns) and state8 (optimizer states in 8 bits). ``install()`` points transformer_lm.sol_modules at
   these classes so that train_sol.py runs unchanged.
 """
+from . import state8
 from .adamw import AdamW
 from .clip import clip_grad_norm_
 from .ema import EmaWeights
 from .normuon import NorMuonGNS
 from .routing import build_optimizers, route_params
 
-__all__ = ["AdamW", "EmaWeights", "NorMuonGNS", "build_optimizers", "clip_grad_norm_", "route_params", "install"]
+__all__ = ["AdamW", "EmaWeights", "NorMuonGNS", "build_optimizers", "clip_grad_norm_", "route_params", "install",
+           "state8"]
 
 
 def install(module=None):

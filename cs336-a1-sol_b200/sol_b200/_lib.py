@@ -53,6 +53,51 @@ class AdamwGroup(C.Structure):
     ]
 
 
+class Adamw8Tensor(C.Structure):
+    """b2o_adamw8_tensor: a tensor whose moments are held in 8 bits."""
+    _fields_ = [
+        ("param", c_void_p),
+        ("rem", c_void_p),
+        ("grad", c_void_p),
+        ("exp_avg", c_void_p),
+        ("exp_avg_sq", c_void_p),
+        ("exp_avg_scale", c_void_p),
+        ("exp_avg_sq_scale", c_void_p),
+        ("ema", c_void_p),
+        ("numel", c_int64),
+        ("first", c_int64),
+        ("group", C.c_int32),
+        ("_pad", C.c_int32),
+        ("step_out", c_void_p),
+    ]
+
+
+class Adamw8Group(C.Structure):
+    _fields_ = [
+        ("lr", C.c_double),
+        ("beta1", C.c_double),
+        ("beta2", C.c_double),
+        ("eps", C.c_double),
+        ("weight_decay", C.c_double),
+        ("step", C.c_double),
+        ("grad_scale", c_void_p),
+        ("cautious", C.c_int32),
+        ("_pad", C.c_int32),
+    ]
+
+
+class StateTensor(C.Structure):
+    """b2o_state_tensor: one state of an encode or decode call."""
+    _fields_ = [
+        ("value", c_void_p),
+        ("codes", c_void_p),
+        ("scales", c_void_p),
+        ("numel", c_int64),
+        ("kind", C.c_int32),
+        ("value_dtype", C.c_int32),
+    ]
+
+
 class NormuonBatch(C.Structure):
     """b2o_normuon_batch: one shape batch of a multi-batch front/apply call."""
     _fields_ = [
@@ -106,6 +151,11 @@ SIGNATURES = {
     "b2o_gemm_timing_read": (c_int, [C.POINTER(C.c_double), C.POINTER(C.c_double), C.POINTER(c_int64)]),
     "b2o_adamw_step": (c_int, [C.POINTER(AdamwTensor), c_int, C.POINTER(AdamwGroup), c_int, c_int, c_int,
                                c_float, c_void_p]),
+    "b2o_state_blocks": (c_int64, [c_int64]),
+    "b2o_state_encode": (c_int, [C.POINTER(StateTensor), c_int, c_void_p]),
+    "b2o_state_decode": (c_int, [C.POINTER(StateTensor), c_int, c_void_p]),
+    "b2o_adamw8_step": (c_int, [C.POINTER(Adamw8Tensor), c_int, C.POINTER(Adamw8Group), c_int, c_int, c_float,
+                                c_void_p]),
     "b2o_ema_update": (c_int, [C.POINTER(c_void_p), C.POINTER(c_void_p), C.POINTER(c_int64), c_int, c_int,
                                c_float, c_void_p]),
     "b2o_ema_copy_to_params": (c_int, [C.POINTER(c_void_p), C.POINTER(c_void_p), C.POINTER(c_int64), c_int,
@@ -142,6 +192,10 @@ SIGNATURES = {
                                         c_void_p]),
     "b2o_normuon_prescale": (c_int, [C.POINTER(NormuonBatch), c_int, c_int, c_float, c_float, c_int, c_void_p,
                                      c_float, c_float, c_void_p]),
+    "b2o_normuon_front8_multi": (c_int, [C.POINTER(NormuonBatch), C.POINTER(c_void_p), C.POINTER(c_void_p), c_int,
+                                         c_int, C.c_double, c_int, c_void_p, c_void_p]),
+    "b2o_normuon_prescale8": (c_int, [C.POINTER(NormuonBatch), C.POINTER(c_void_p), c_int, c_int, C.c_double, c_int,
+                                      c_void_p, c_float, c_float, c_void_p]),
     "b2o_clip_scratch_floats": (c_int64, [C.POINTER(c_int64), c_int]),
     "b2o_clip_grad_norm": (c_int, [C.POINTER(c_void_p), C.POINTER(c_int64), C.POINTER(c_int), c_int, c_float,
                                    c_void_p, c_void_p, c_void_p]),
@@ -198,6 +252,21 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class on_device:
+    """Makes ``device`` current for a launch (free where it already is)."""
+
+    def __init__(self, device: torch.device):
+        self._ctx = None if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._ctx is not None:
+            self._ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
 
 
 def ptr_array(ptrs) -> C.Array:

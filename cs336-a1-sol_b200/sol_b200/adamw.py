@@ -6,13 +6,22 @@ defaults, param-group keys (lr, betas, eps, weight_decay, amsgrad, maximize,
 foreach, capturable, differentiable, fused) and per-parameter state
 (``step`` fp32 0-d tensor, ``exp_avg``, ``exp_avg_sq``).
 
-Two storage modes:
+Storage modes:
   * reference (default): moments in the parameter dtype, exactly what torch's
     fused AdamW keeps for bf16 parameters; the arithmetic is torch's fused
     formula (ATen/native/cuda/fused_adam_utils.cuh, ADAMW mode) in fp32.
   * master="bf16_mt": bf16 parameter plus a bf16 low-mantissa remainder
     (``mant_rem``, the NorMuonGNS trick at sol_modules.py:406-424) and fp32
     moments (state_dtype=torch.float32); optional cautious weight decay.
+  * state_dtype=torch.int8 (with either of the above): both moments in 8 bits
+    with one fp32 scale per 128 elements (format in state8.py; state keys
+    ``exp_avg`` int8, ``exp_avg_sq`` uint8, ``exp_avg_scale``,
+    ``exp_avg_sq_scale``): 2.06 bytes per element instead of 4 or 8, and 22
+    bytes moved per element of the recipe's tables instead of 34. Parameters
+    with fewer than ``min_8bit_numel`` elements (gains, gates, scalars: nothing
+    to save there) keep fp32 moments. The rounding is even over steps and a
+    function of element and step alone, so results repeat and a sharded step
+    gives what one GPU gives.
 One streaming kernel pass updates parameter, remainder, moments and (when an
 EmaWeights object has armed folding) the fp32 EMA shadow.
 """
@@ -23,7 +32,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, state8
 from .ema import register_optimizer
 
 MAX_GROUPS = 8
@@ -31,12 +40,15 @@ MAX_GROUPS = 8
 _DESC_WORDS = C.sizeof(_lib.AdamwTensor) // 8
 _GRAD_WORD = _lib.AdamwTensor.grad.offset // 8
 assert C.sizeof(_lib.AdamwTensor) % 8 == 0 and _lib.AdamwTensor.grad.offset % 8 == 0
+_DESC8_WORDS = C.sizeof(_lib.Adamw8Tensor) // 8
+_GRAD8_WORD = _lib.Adamw8Tensor.grad.offset // 8
 
 
 class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False, *,
                  maximize=False, foreach=None, capturable=False, differentiable=False, fused=None,
-                 decoupled_weight_decay=True, master="none", state_dtype=None, cautious_wd=False):
+                 decoupled_weight_decay=True, master="none", state_dtype=None, cautious_wd=False,
+                 min_8bit_numel=4096):
         if amsgrad or maximize or capturable or differentiable or not decoupled_weight_decay:
             raise ValueError("the B200 AdamW implements the recipe's configuration: no amsgrad/maximize/"
                              "capturable/differentiable")
@@ -46,7 +58,13 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, defaults)
         if master not in ("none", "bf16_mt"):
             raise ValueError("master must be 'none' or 'bf16_mt'")
+        if state_dtype not in (None, torch.float32, torch.bfloat16, torch.int8):
+            raise ValueError("state_dtype must be None, torch.float32, torch.bfloat16 or torch.int8")
+        if state_dtype == torch.int8:
+            for group in self.param_groups:
+                self._check_8bit_group(group)
         self.master = master
+        self.min_8bit_numel = int(min_8bit_numel)
         self.state_dtype = state_dtype
         self.cautious_wd = cautious_wd
         self._steps = {}           # id(param) -> int step count (mirrors state["step"])
@@ -57,11 +75,31 @@ class AdamW(torch.optim.Optimizer):
         self._plan = None          # cached launch descriptors (see step)
         register_optimizer(self)
 
+    @staticmethod
+    def _check_8bit_group(group):
+        b1, b2 = group["betas"]
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and group["eps"] >= 0.0):
+            raise ValueError("AdamW with 8-bit moments needs betas in [0, 1) and eps >= 0")
+
+    def holds_8bit(self, p) -> bool:
+        """Whether this optimizer keeps p's moments in 8 bits."""
+        return self.state_dtype == torch.int8 and p.numel() >= max(1, self.min_8bit_numel)
+
     def _init_state(self, p):
         st = self.state[p]
+        if "step" not in st and self.holds_8bit(p):
+            st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+            nb = state8.blocks(p.numel())
+            st["exp_avg"] = torch.zeros_like(p, dtype=torch.int8, memory_format=torch.preserve_format)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
+            st["exp_avg_scale"] = torch.zeros(nb, dtype=torch.float32, device=p.device)
+            st["exp_avg_sq_scale"] = torch.zeros(nb, dtype=torch.float32, device=p.device)
+            if self.master == "bf16_mt" and p.dtype == torch.bfloat16:
+                st["mant_rem"] = torch.zeros_like(p)
+            self._steps[id(p)] = 0
         if "step" not in st:
             st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
-            sdt = self.state_dtype or p.dtype
+            sdt = torch.float32 if self.state_dtype == torch.int8 else self.state_dtype or p.dtype
             if self.master == "bf16_mt" and p.dtype == torch.bfloat16 and self.state_dtype is None:
                 sdt = torch.float32
             st["exp_avg"] = torch.zeros_like(p, dtype=sdt, memory_format=torch.preserve_format)
@@ -74,15 +112,88 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Keeps each saved state tensor's dtype (fp32 moments of bf16 parameters
-        in master mode; torch's loader would cast them to bf16)."""
+        in master mode; torch's loader would cast them to bf16), except between
+        8-bit and wider moments: those are converted to what this optimizer
+        holds (on the GPU; needs the parameters there)."""
         from .normuon import _load_state_keep_dtypes
         _load_state_keep_dtypes(self, state_dict)
         self._plan = None
+        self._convert_loaded()
         for group in self.param_groups:
             for p in group["params"]:
                 st = self.state.get(p)
                 if st and "step" in st:
                     self._steps[id(p)] = int(float(st["step"].item()))
+
+    def _convert_loaded(self):
+        narrow, widen = [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                st = self.state.get(p)
+                if not st or "exp_avg" not in st:
+                    continue
+                if self.holds_8bit(p) and st["exp_avg"].dtype != torch.int8:
+                    narrow.append(st)
+                elif not self.holds_8bit(p) and st["exp_avg"].dtype == torch.int8:
+                    widen.append((p, st))
+        if narrow:
+            kept = state8.encode([x for st in narrow for x in ((st["exp_avg"].contiguous(), "signed"),
+                                                               (st["exp_avg_sq"].contiguous(), "root"))])
+            for i, st in enumerate(narrow):
+                st["exp_avg"], st["exp_avg_scale"] = kept[2 * i]
+                st["exp_avg_sq"], st["exp_avg_sq_scale"] = kept[2 * i + 1]
+        for p, st in widen:
+            dt = self.state_dtype if self.state_dtype in (torch.float32, torch.bfloat16) else torch.float32
+            if self.state_dtype is None and self.master == "none":
+                dt = p.dtype
+            st["exp_avg"], st["exp_avg_sq"] = state8.decode(
+                [(st["exp_avg"], st.pop("exp_avg_scale"), "signed"),
+                 (st["exp_avg_sq"], st.pop("exp_avg_sq_scale"), "root")], dtype=dt)
+
+    @torch.no_grad()
+    def expanded_state(self, params=None, dtype=torch.float32):
+        """The moments as ``dtype`` (fp32 or bf16) tensors, and the fp32 master
+        weight where a bf16 parameter has a remainder: one dict per parameter
+        with "exp_avg", "exp_avg_sq" and, there, "master". 8-bit moments and
+        master weights of all parameters are expanded in one launch; moments
+        that are wide already are cast by torch. (In a sharded step a rank's
+        moments are those of its own rows until ``gather_state``.)"""
+        if params is None:
+            params = [p for g in self.param_groups for p in g["params"]]
+        items, dts, out, where = [], [], [], []
+        for i, p in enumerate(params):
+            _lib.require_cuda(p, "AdamW.expanded_state")
+            st = self._init_state(p)
+            out.append({})
+            if st["exp_avg"].dtype == torch.int8:
+                items += [(st["exp_avg"], st["exp_avg_scale"], "signed"), (st["exp_avg_sq"], st["exp_avg_sq_scale"], "root")]
+                dts += [dtype, dtype]
+                where += [(i, "exp_avg"), (i, "exp_avg_sq")]
+            else:
+                out[i]["exp_avg"] = st["exp_avg"].to(dtype, copy=True)
+                out[i]["exp_avg_sq"] = st["exp_avg_sq"].to(dtype, copy=True)
+            if "mant_rem" in st:
+                items.append((p.detach(), st["mant_rem"], "pair"))
+                dts.append(torch.float32)
+                where.append((i, "master"))
+        for (i, key), v in zip(where, state8.decode(items, dtype=dts)):
+            out[i][key] = v
+        return out
+
+    def expanded_state_dict(self):
+        """state_dict() with 8-bit moments expanded to fp32 (the layout of torch's AdamW)."""
+        sd = self.state_dict()
+        for p, key in self._state_keys(sd):
+            st = sd["state"].get(key)
+            if st and "exp_avg" in st and st["exp_avg"].dtype == torch.int8:
+                wide = self.expanded_state([p])[0]
+                sd["state"][key] = {k: wide.get(k, v) for k, v in st.items()
+                                    if k not in ("exp_avg_scale", "exp_avg_sq_scale")}
+        return sd
+
+    def _state_keys(self, sd):
+        params = [p for g in self.param_groups for p in g["params"]]
+        return list(zip(params, [k for g in sd["param_groups"] for k in g["params"]]))
 
     def invalidate_plan(self) -> None:
         """Drops the cached launch descriptors (rebuilt on the next step). Needed
@@ -108,7 +219,7 @@ class AdamW(torch.optim.Optimizer):
             buckets.setdefault((p.device, p.dtype, st["exp_avg"].dtype), []).append((gi, p, st))
         launches, ema_idx = [], set()
         pos = {id(p): i for i, p in enumerate(ps)}
-        # (word view of a descriptor array, its rows, the items' positions in ps, byte offsets)
+        # (gradient words of a descriptor array, the items' positions in ps, byte offsets)
         refresh = []
         for (dev, pdt, sdt), members in buckets.items():
             descs, owners = [], []
@@ -123,30 +234,60 @@ class AdamW(torch.optim.Optimizer):
                     start, n = sl
                 esz = p.element_size()
                 ssz = st["exp_avg"].element_size()
-                descs.append(_lib.AdamwTensor(
-                    p.data_ptr() + start * esz,
-                    (rem.data_ptr() + start * 2) if rem is not None else None,
-                    None,
-                    st["exp_avg"].data_ptr() + start * ssz,
-                    st["exp_avg_sq"].data_ptr() + start * ssz,
-                    (shadow.data_ptr() + start * 4) if shadow is not None else None,
-                    n, gi, 0, st["step"].data_ptr()))
+                if sdt == torch.int8:
+                    if start % state8.BLOCK or ((start + n) % state8.BLOCK and start + n != p.numel()):
+                        raise ValueError("AdamW: a slice of 8-bit moments starts and ends at multiples of "
+                                         f"{state8.BLOCK} elements (got {start}, {n} of {p.numel()})")
+                    sc = 4 * (start // state8.BLOCK)
+                    descs.append(_lib.Adamw8Tensor(
+                        p.data_ptr() + start * esz,
+                        (rem.data_ptr() + start * 2) if rem is not None else None,
+                        None,
+                        st["exp_avg"].data_ptr() + start,
+                        st["exp_avg_sq"].data_ptr() + start,
+                        st["exp_avg_scale"].data_ptr() + sc,
+                        st["exp_avg_sq_scale"].data_ptr() + sc,
+                        (shadow.data_ptr() + start * 4) if shadow is not None else None,
+                        n, start, gi, 0, st["step"].data_ptr()))
+                else:
+                    descs.append(_lib.AdamwTensor(
+                        p.data_ptr() + start * esz,
+                        (rem.data_ptr() + start * 2) if rem is not None else None,
+                        None,
+                        st["exp_avg"].data_ptr() + start * ssz,
+                        st["exp_avg_sq"].data_ptr() + start * ssz,
+                        (shadow.data_ptr() + start * 4) if shadow is not None else None,
+                        n, gi, 0, st["step"].data_ptr()))
                 owners.append((p, start * esz))
                 if shadow is not None:
                     ema_idx.add(self._ema._index[id(p)])
             if not descs:
                 continue
-            arr = (_lib.AdamwTensor * len(descs))(*descs)
-            words = np.frombuffer(arr, dtype=np.uint64).reshape(len(descs), _DESC_WORDS)
-            refresh.append((words, np.array([pos[id(p)] for p, _ in owners]),
+            eight = sdt == torch.int8
+            arr = ((_lib.Adamw8Tensor if eight else _lib.AdamwTensor) * len(descs))(*descs)
+            words = np.frombuffer(arr, dtype=np.uint64).reshape(len(descs), _DESC8_WORDS if eight else _DESC_WORDS)
+            refresh.append((words[:, _GRAD8_WORD if eight else _GRAD_WORD], np.array([pos[id(p)] for p, _ in owners]),
                             np.array([off for _, off in owners], dtype=np.uint64)))
-            launches.append((arr, len(descs), _lib.dtype_code(pdt), _lib.dtype_code(sdt), _lib.stream_ptr(dev)))
+            launches.append((arr, len(descs), _lib.dtype_code(pdt), None if eight else _lib.dtype_code(sdt), dev))
         by_group = {}
         for gi, p in zip(gis, ps):
             by_group.setdefault(gi, []).append(id(p))
         return {"key": key, "ema": self._ema, "owned": self._owned_slices, "state": self.state,
                 "keep": ps, "launches": launches, "refresh": refresh, "groups": by_group,
                 "ema_idx": frozenset(ema_idx)}
+
+    def _groups8(self, steps_of, grad_scale):
+        """Group table of the 8-bit pass; a group that does not step gets a neutral row."""
+        tab = (_lib.Adamw8Group * max(1, len(self.param_groups)))()
+        for gi, group in enumerate(self.param_groups):
+            if gi not in steps_of:
+                tab[gi].step = 1.0
+                continue
+            b1, b2 = group["betas"]
+            tab[gi] = _lib.Adamw8Group(float(group["lr"]), float(b1), float(b2), float(group["eps"]),
+                                       float(group["weight_decay"]), float(steps_of[gi]), grad_scale,
+                                       int(bool(self.cautious_wd)))
+        return tab
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -167,6 +308,9 @@ class AdamW(torch.optim.Optimizer):
                     ps.append(p)
                     gs_.append(g)
                     gis.append(gi)
+        if self.state_dtype == torch.int8:
+            for gi in set(gis):
+                self._check_8bit_group(self.param_groups[gi])
         # The launch descriptors depend only on which parameters step, where
         # their storage and state live, the EMA folding and the shard: cached
         # across steps; the gradient pointers are written into them each step.
@@ -177,7 +321,7 @@ class AdamW(torch.optim.Optimizer):
             plan = self._plan = self._build_plan(ps, gis, key)
         gptr = np.fromiter((g.data_ptr() for g in gs_), dtype=np.uint64, count=len(gs_))
         for words, where, offs in plan["refresh"]:
-            words[:, _GRAD_WORD] = gptr[where] + offs
+            words[:] = gptr[where] + offs
         steps_of = {}
         for gi, ids in plan["groups"].items():
             k = self._steps.get(ids[0], 0) + 1
@@ -199,9 +343,18 @@ class AdamW(torch.optim.Optimizer):
         for i, g in enumerate(gtab):
             if g is not None:
                 groups[i] = g
-        for arr, n, pdt, sdt, stream in plan["launches"]:
-            rc = lib.b2o_adamw_step(arr, n, groups, len(gtab), pdt, sdt, self._ema_weight, stream)
-            _lib.check(rc, "adamw_step")
+        groups8 = None
+        for arr, n, pdt, sdt, dev in plan["launches"]:
+            with _lib.on_device(dev):
+                if sdt is None:
+                    if groups8 is None:
+                        groups8 = self._groups8(steps_of, gsc)
+                    rc = lib.b2o_adamw8_step(arr, n, groups8, len(gtab), pdt, self._ema_weight, _lib.stream_ptr(dev))
+                    _lib.check(rc, "adamw8_step")
+                else:
+                    rc = lib.b2o_adamw_step(arr, n, groups, len(gtab), pdt, sdt, self._ema_weight,
+                                            _lib.stream_ptr(dev))
+                    _lib.check(rc, "adamw_step")
         if self._ema is not None and plan["ema_idx"]:
             self._ema._folded |= plan["ema_idx"]
         self._grad_scale = None

@@ -28,15 +28,21 @@ def _rank0(sharded) -> bool:
     return sharded is None or sharded.world == 1 or sharded.rank == 0
 
 
-def save_checkpoint(model, optimizer, iteration, out, *, adamw=None, sharded=None):
+def save_checkpoint(model, optimizer, iteration, out, *, adamw=None, sharded=None, expand_state=False):
     """modules.py:538-550 layout (+ "adamw"). With ``sharded``, call on every
-    rank; rank 0 writes."""
+    rank; rank 0 writes. ``expand_state``: write states held in 8 bits as wide
+    tensors (the NorMuon momentum in the parameter dtype, AdamW's moments in
+    fp32), for readers without them, the reference's loader among them; the
+    engine's own loaders take either form."""
     if sharded is not None:
         sharded.gather_state()
     if _rank0(sharded):
-        obj = {"model": _unwrap(model).state_dict(), "optimizer": optimizer.state_dict(), "iteration": iteration}
+        def state(opt):
+            return opt.expanded_state_dict() if expand_state else opt.state_dict()
+
+        obj = {"model": _unwrap(model).state_dict(), "optimizer": state(optimizer), "iteration": iteration}
         if adamw is not None:
-            obj["adamw"] = adamw.state_dict()
+            obj["adamw"] = state(adamw)
         torch.save(obj, out)
     if sharded is not None:
         sharded.drop_unowned_state()

@@ -27,7 +27,7 @@ from collections import OrderedDict
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, state8
 from .ema import register_optimizer
 from .polar_express import table_for
 
@@ -55,15 +55,26 @@ class NorMuonGNS(torch.optim.Optimizer):
           zeropower_via_newtonschulz5, restated on the same GEMM engine).
       coefficients: "polar_express" or "quintic" coefficient table for "gram".
       reset_iterations: Gram restart steps (the reference passes [2], :357).
+      momentum_dtype: None (parameter dtype, as the reference) or torch.int8: the
+          momentum in 8 bits with one fp32 scale per 128 elements (format in
+          state8.py); state keys ``momentum_buffer`` int8 (r, c),
+          ``momentum_scale`` and ``momentum_step`` (the step count that the
+          rounding of the codes runs with).
     """
 
     def __init__(self, params, lr=2e-3, momentum=0.95, beta2=0.95, nesterov=True, ns_steps=5,
                  weight_decay=0.0, cautious_wd=False, bf16_master=False, *, orthogonalizer="gram",
-                 coefficients="polar_express", reset_iterations=(2,), norm_eps=1e-7, norm_safety=1.0):
+                 coefficients="polar_express", reset_iterations=(2,), norm_eps=1e-7, norm_safety=1.0,
+                 momentum_dtype=None):
         super().__init__(params, dict(lr=lr, momentum=momentum, beta2=beta2, nesterov=nesterov,
                                       ns_steps=ns_steps, weight_decay=weight_decay))
         if orthogonalizer not in ("gram", "quintic"):
             raise ValueError("orthogonalizer must be 'gram' or 'quintic'")
+        if momentum_dtype not in (None, torch.int8):
+            raise ValueError("momentum_dtype must be None or torch.int8")
+        if momentum_dtype == torch.int8 and not all(0.0 <= g["momentum"] < 1.0 for g in self.param_groups):
+            raise ValueError("NorMuonGNS with an 8-bit momentum needs momentum in [0, 1)")
+        self.momentum_dtype = momentum_dtype
         self.cautious_wd = cautious_wd
         self.bf16_master = bf16_master
         self.orthogonalizer = orthogonalizer
@@ -158,9 +169,50 @@ class NorMuonGNS(torch.optim.Optimizer):
         """Loads param groups and per-parameter state keeping each saved tensor's
         dtype (torch's Optimizer.load_state_dict casts floating-point state to the
         parameter dtype, which would turn the fp32 v_row of bf16 matrices into
-        bf16)."""
+        bf16), except between an 8-bit momentum and a wide one: those are
+        converted to what this optimizer holds (on the GPU; needs the parameters
+        there)."""
         _load_state_keep_dtypes(self, state_dict)
         self._plans = {}
+        self._convert_loaded()
+
+    def _convert_loaded(self):
+        narrow, widen = [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                st = self.state.get(p)
+                if not st or "momentum_buffer" not in st:
+                    continue
+                eight = st["momentum_buffer"].dtype == torch.int8
+                if self.momentum_dtype == torch.int8 and not eight:
+                    narrow.append(st)
+                elif self.momentum_dtype is None and eight:
+                    widen.append((p, st))
+        if narrow:
+            kept = state8.encode([(st["momentum_buffer"].contiguous(), "signed") for st in narrow])
+            for st, (codes, scales) in zip(narrow, kept):
+                st["momentum_buffer"], st["momentum_scale"], st["momentum_step"] = codes, scales, 0
+        if widen:
+            vals = state8.decode([(st["momentum_buffer"], st.pop("momentum_scale"), "signed") for _, st in widen],
+                                 dtype=[p.dtype for p, _ in widen])
+            for (_, st), v in zip(widen, vals):
+                st["momentum_buffer"] = v
+                st.pop("momentum_step", None)
+
+    def expanded_state_dict(self):
+        """state_dict() with an 8-bit momentum expanded to the parameter dtype
+        (the reference's layout)."""
+        sd = self.state_dict()
+        params = [p for g in self.param_groups for p in g["params"]]
+        found = [(p, k) for p, k in zip(params, [k for g in sd["param_groups"] for k in g["params"]])
+                 if "momentum_scale" in sd["state"].get(k, {})]
+        vals = state8.decode([(sd["state"][k]["momentum_buffer"], sd["state"][k]["momentum_scale"], "signed")
+                              for _, k in found], dtype=[p.dtype for p, _ in found])
+        for (_, k), v in zip(found, vals):
+            st = {n: x for n, x in sd["state"][k].items() if n not in ("momentum_scale", "momentum_step")}
+            st["momentum_buffer"] = v
+            sd["state"][k] = st
+        return sd
 
     def _hook_overridden(self):
         return ("_orthogonalize_batch" in self.__dict__ or
@@ -169,7 +221,12 @@ class NorMuonGNS(torch.optim.Optimizer):
     def _init_state(self, p):
         st = self.state[p]
         if "momentum_buffer" not in st:
-            st["momentum_buffer"] = torch.zeros_like(p)
+            if self.momentum_dtype == torch.int8:
+                st["momentum_buffer"] = torch.zeros_like(p, dtype=torch.int8)
+                st["momentum_scale"] = torch.zeros(state8.blocks(p.numel()), dtype=torch.float32, device=p.device)
+                st["momentum_step"] = 0
+            else:
+                st["momentum_buffer"] = torch.zeros_like(p)
             st["v_row"] = torch.zeros_like(p[..., 0:1], dtype=torch.float32)
         if self.bf16_master and p.dtype == torch.bfloat16 and "mant_rem" not in st:
             st["mant_rem"] = torch.zeros_like(p)
@@ -213,6 +270,37 @@ class NorMuonGNS(torch.optim.Optimizer):
             if cur:
                 yield k, cur
 
+    def _momentum8(self, members):
+        """Scale pointer and step tables of a front call with 8-bit momenta (None
+        without): the tables, the states whose step counts they carry, and what
+        keeps them alive."""
+        if self.momentum_dtype is None:
+            return None
+        scales = [_lib.ptr_array([st["momentum_scale"].data_ptr() for st in b["states"]]) for b in members]
+        steps = [np.zeros(b["S"], dtype=np.uint32) for b in members]
+        return (_lib.ptr_array([_lib.addr(x) for x in scales]), _lib.ptr_array([x.ctypes.data for x in steps]),
+                [(x, b["states"]) for x, b in zip(steps, members)], scales)
+
+    def _front_call(self, lib, arr, n, dtc, beta, nesterov, gs, dev, x0, m8):
+        stream = _lib.stream_ptr(dev)
+        if m8 is None:
+            args = (arr, n, dtc, 1.0 - beta, beta, nesterov, gs)
+            _lib.check(lib.b2o_normuon_front_multi(*args, stream), "normuon_front")
+            if x0:
+                _lib.check(lib.b2o_normuon_prescale(*args, self.norm_eps, self.norm_safety, stream),
+                           "normuon_prescale")
+            return
+        scales, step_ptrs, counts, _ = m8
+        for table, states in counts:
+            for j, st in enumerate(states):
+                st["momentum_step"] += 1
+                table[j] = st["momentum_step"] & 0xFFFFFFFF
+        _lib.check(lib.b2o_normuon_front8_multi(arr, scales, step_ptrs, n, dtc, beta, nesterov, gs, stream),
+                   "normuon_front8")
+        if x0:
+            _lib.check(lib.b2o_normuon_prescale8(arr, scales, n, dtc, beta, nesterov, gs, self.norm_eps,
+                                                 self.norm_safety, stream), "normuon_prescale8")
+
     def _front_all(self, recs, group):
         """Momentum + Nesterov (sol_modules.py:390-394) for every batch: one launch per call."""
         lib = _lib.load()
@@ -220,6 +308,7 @@ class NorMuonGNS(torch.optim.Optimizer):
         for (dev, dt), members in self._calls(recs, lambda b: (b["dev"], b["params"][0].dtype)):
             arr = (_lib.NormuonBatch * len(members))()
             keep = []
+            m8 = self._momentum8(members)
             for i, b in enumerate(members):
                 grads = _lib.ptr_array([p.grad.data_ptr() for p in b["params"]])
                 bufs = _lib.ptr_array([st["momentum_buffer"].data_ptr() for st in b["states"]])
@@ -231,11 +320,8 @@ class NorMuonGNS(torch.optim.Optimizer):
                                            xscale=ws["xscale"].data_ptr(), flags=ws["flags"].data_ptr(),
                                            x0_half=int(b["x0"]))
             gs = self._grad_scale.data_ptr() if self._grad_scale is not None else None
-            args = (arr, len(members), _lib.dtype_code(dt), 1.0 - beta, beta, int(bool(group["nesterov"])), gs)
-            _lib.check(lib.b2o_normuon_front_multi(*args, _lib.stream_ptr(dev)), "normuon_front")
-            if any(b["x0"] for b in members):
-                _lib.check(lib.b2o_normuon_prescale(*args, self.norm_eps, self.norm_safety, _lib.stream_ptr(dev)),
-                           "normuon_prescale")
+            self._front_call(lib, arr, len(members), _lib.dtype_code(dt), beta, int(bool(group["nesterov"])), gs, dev,
+                             any(b["x0"] for b in members), m8)
 
     def _ortho_class(self, batches, ns_steps):
         """Orthogonalises every batch of one m = min(r, c) class with one library call."""
@@ -367,8 +453,8 @@ class NorMuonGNS(torch.optim.Optimizer):
                                            partial=ws["partial"].data_ptr(), prescale=ws["prescale"].data_ptr(),
                                            xscale=ws["xscale"].data_ptr(), flags=ws["flags"].data_ptr(),
                                            x0_half=int(b["x0"]))
-            front.append((arr, len(members), _lib.dtype_code(dt), _lib.stream_ptr(dev),
-                          any(b["x0"] for b in members)))
+            front.append((arr, len(members), _lib.dtype_code(dt), dev, any(b["x0"] for b in members),
+                          self._momentum8(members)))
         ortho = []
         classes = OrderedDict()
         for b in recs:
@@ -383,7 +469,7 @@ class NorMuonGNS(torch.optim.Optimizer):
             okey = ("multi",) + tuple((b["S"], b["r"], b["c"]) for b in members)
             nbytes = lib.b2o_ortho_workspace_bytes_multi(groups, len(members))
             wsb = self._ortho_ws(dev, okey, nbytes)
-            ortho.append((groups, len(members), wsb, _lib.stream_ptr(dev), m))
+            ortho.append((groups, len(members), wsb, dev, m))
         apply, ema_idx = [], set()
 
         def akey(b):
@@ -409,7 +495,7 @@ class NorMuonGNS(torch.optim.Optimizer):
                                            o=ws["o"].data_ptr(), rowsq=ws["rowsq"].data_ptr(),
                                            params=_lib.addr(pptr), rems=_lib.addr(rems), emas=_lib.addr(emas),
                                            vrows=_lib.addr(vrows), scratch=ws["scratch"].data_ptr())
-            apply.append((arr, len(members), _lib.dtype_code(dt), _lib.stream_ptr(dev)))
+            apply.append((arr, len(members), _lib.dtype_code(dt), dev))
         states = [self.state[p] for p in params]
         return {"key": key, "ema": self._ema, "owned": self._owned, "state": self.state,
                 "keep": (keep, params, states, recs, gflat), "front": front, "ortho": ortho, "apply": apply,
@@ -423,23 +509,19 @@ class NorMuonGNS(torch.optim.Optimizer):
         beta = float(group["momentum"])
         nesterov = int(bool(group["nesterov"]))
         gs = self._grad_scale.data_ptr() if self._grad_scale is not None else None
-        for arr, n, dtc, stream, x0 in plan["front"]:
-            args = (arr, n, dtc, 1.0 - beta, beta, nesterov, gs)
-            _lib.check(lib.b2o_normuon_front_multi(*args, stream), "normuon_front")
-            if x0:
-                _lib.check(lib.b2o_normuon_prescale(*args, self.norm_eps, self.norm_safety, stream),
-                           "normuon_prescale")
+        for arr, n, dtc, dev, x0, m8 in plan["front"]:
+            self._front_call(lib, arr, n, dtc, beta, nesterov, gs, dev, x0, m8)
         ns_steps = int(group["ns_steps"])
         coeffs, resets, nres = self._table(ns_steps)
         mode = 0 if self.orthogonalizer == "quintic" else 1
         ev = self._timing_events
-        for groups, n, wsb, stream, m in plan["ortho"]:
+        for groups, n, wsb, dev, m in plan["ortho"]:
             if ev is not None:
                 e0 = torch.cuda.Event(enable_timing=True)
                 e0.record()
                 n0 = _lib.launch_count()
             rc = lib.b2o_orthogonalize_multi(groups, n, mode, coeffs, ns_steps, resets, nres, self.norm_eps,
-                                             self.norm_safety, wsb.data_ptr(), wsb.numel(), stream)
+                                             self.norm_safety, wsb.data_ptr(), wsb.numel(), _lib.stream_ptr(dev))
             _lib.check(rc, "orthogonalize_multi")
             if ev is not None:
                 e1 = torch.cuda.Event(enable_timing=True)
@@ -447,10 +529,10 @@ class NorMuonGNS(torch.optim.Optimizer):
                 ev.append((e0, e1, m, _lib.launch_count() - n0))
         beta2 = float(group["beta2"])
         lr, wd = float(group["lr"]), float(group["weight_decay"])
-        for arr, n, dtc, stream in plan["apply"]:
+        for arr, n, dtc, dev in plan["apply"]:
             rc = lib.b2o_normuon_apply_multi(arr, n, dtc, -lr, lr * wd, 1.0 - lr * wd, 1 if wd else 0,
                                              int(bool(self.cautious_wd and wd)), 1.0 - beta2, self._ema_weight,
-                                             stream)
+                                             _lib.stream_ptr(dev))
             _lib.check(rc, "normuon_apply")
         if self._ema is not None and plan["ema_idx"]:
             self._ema._folded |= plan["ema_idx"]

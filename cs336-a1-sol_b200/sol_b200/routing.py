@@ -48,8 +48,10 @@ def build_optimizers(model, *, muon_lr: float, adam_lr: float, embed_lr: float, 
                      betas=(0.9, 0.95), eps=1e-8, cautious_wd: bool = False, bf16_master: bool = False,
                      ve_lr: float | None = None, orthogonalizer: str = "gram",
                      coefficients: str = "polar_express", adam_master: str = "none", adam_state_dtype=None,
-                     adam_cautious_wd: bool = False):
-    """Reference signature plus engine options (orthogonaliser and AdamW storage mode)."""
+                     adam_cautious_wd: bool = False, momentum_dtype=None):
+    """Reference signature plus engine options (orthogonaliser and storage modes:
+    adam_state_dtype=torch.int8 and momentum_dtype=torch.int8 keep the AdamW
+    moments and the NorMuon momentum in 8 bits)."""
     inner = getattr(model, "_orig_mod", model)
     muon_params, embed_params, norm_params, ve_params = route_params(inner.named_parameters())
     groups = []
@@ -63,7 +65,8 @@ def build_optimizers(model, *, muon_lr: float, adam_lr: float, embed_lr: float, 
     adamw = AdamW(groups, betas=betas, eps=eps, fused=True, master=adam_master, state_dtype=adam_state_dtype,
                   cautious_wd=adam_cautious_wd)
     muon = NorMuonGNS(muon_params, lr=muon_lr, weight_decay=weight_decay, cautious_wd=cautious_wd,
-                      bf16_master=bf16_master, orthogonalizer=orthogonalizer, coefficients=coefficients)
+                      bf16_master=bf16_master, orthogonalizer=orthogonalizer, coefficients=coefficients,
+                      momentum_dtype=momentum_dtype)
     for opt in (muon, adamw):
         for g in opt.param_groups:
             g["base_lr"] = g["lr"]

@@ -32,7 +32,7 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 
-from . import _lib
+from . import _lib, state8
 
 
 def gram_cost(shape) -> float:
@@ -257,7 +257,9 @@ class ShardedStep:
         for g in adamw.param_groups:
             for p in g["params"]:
                 rows = p.shape[0] if p.dim() >= 1 else 0
-                if p.dim() >= 2 and p.numel() >= min_rows_shard * world and p.numel() % world == 0:
+                # a rank's slice of 8-bit moments holds whole blocks
+                unit = state8.BLOCK if adamw.holds_8bit(p) else 1
+                if p.dim() >= 2 and p.numel() >= min_rows_shard * world and p.numel() % (world * unit) == 0:
                     per = p.numel() // world
                     slices[id(p)] = (rank * per, per)
                     self.row_sharded.append(p)
@@ -562,10 +564,15 @@ class ShardedStep:
             for p in g["params"]:
                 st = self.muon._init_state(p)  # zero state where this rank never stepped p
                 for key in sorted(st):
-                    dist.broadcast(st[key], src=self.owner[id(p)], group=self.group)
+                    if torch.is_tensor(st[key]):
+                        dist.broadcast(st[key], src=self.owner[id(p)], group=self.group)
+                    else:  # a step count
+                        n = torch.tensor([st[key]], dtype=torch.int64, device=p.device)
+                        dist.broadcast(n, src=self.owner[id(p)], group=self.group)
+                        st[key] = int(n.item())
         for p in self.row_sharded:
             st = self.adamw._init_state(p)
-            for key in ("exp_avg", "exp_avg_sq", "mant_rem"):
+            for key in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "mant_rem"):
                 if key in st:
                     flat = st[key].view(-1)
                     per = flat.numel() // self.world

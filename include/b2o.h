@@ -105,6 +105,72 @@ int b2o_adamw_step(const b2o_adamw_tensor* tensors, int ntensors,
                    const b2o_adamw_group* groups, int ngroups,
                    int param_dtype, int state_dtype, float ema_weight, void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Optimizer state in 8 bits. A state tensor is cut into blocks of
+ * B2O_STATE_BLOCK consecutive elements (the last may be shorter), each with one
+ * fp32 scale s; b2o_state_blocks(numel) scales per tensor. Kinds:
+ *   SIGNED (first moments, momentum): int8 codes; s = max |x|,
+ *          q = sgn(x) floor(127 sqrt(|x| / s) + u), value s q |q| / 127^2
+ *   ROOT   (second moments, x >= 0): uint8 codes; s = max sqrt(x),
+ *          q = floor(255 sqrt(sqrt(x) / s) + u), at least 1 where x > 0, value (s (q / 255)^2)^2
+ *   PAIR   (bf16 master weights): codes = bf16 weight p = bf16(w), scales =
+ *          bf16 remainder bf16(w - p), value p + remainder; no blocks
+ * u = 1/2 in b2o_state_encode. In a step u runs evenly over [0, 1), so that a
+ * change below a code step is kept on average: for element i of the tensor in
+ * step t, h = 0x9E3779B9 i + 0x6A09E667 t (+ 2^31 for SIGNED) modulo 2^32 and
+ * u = floor(h / 2^9) / 2^23. A block with a value that is not finite (ROOT: or
+ * negative) gets the scale NaN and codes 0, so all of it reads as NaN. A block
+ * of zeros (SIGNED: of magnitudes below 2^-126) gets the scale 0. No reference
+ * counterpart (the reference keeps its states in the parameter dtype).
+ * ------------------------------------------------------------------------ */
+#define B2O_STATE_BLOCK 128
+#define B2O_STATE_SIGNED 0
+#define B2O_STATE_ROOT 1
+#define B2O_STATE_PAIR 2
+int64_t b2o_state_blocks(int64_t numel);
+typedef struct {
+  void* value;          /* encode: read; decode: written; value_dtype, numel elements */
+  void* codes;          /* int8 / uint8 codes, or PAIR: bf16 weight                   */
+  void* scales;         /* fp32 scales, or PAIR: bf16 remainder                       */
+  int64_t numel;
+  int32_t kind;         /* B2O_STATE_*                                                */
+  int32_t value_dtype;  /* B2O_F32 or B2O_BF16                                        */
+} b2o_state_tensor;
+/* value -> codes and scales, and back, for a list of tensors in one launch per
+ * 96 of them. No two tensors of a list may share an output. */
+int b2o_state_encode(const b2o_state_tensor* tensors, int ntensors, void* stream);
+int b2o_state_decode(const b2o_state_tensor* tensors, int ntensors, void* stream);
+
+/* AdamW (+ EMA) as b2o_adamw_step, with both moments in 8 bits: exp_avg SIGNED,
+ * exp_avg_sq ROOT. The update uses the moments before they are rounded to 8
+ * bits. A tensor may be a slice of a larger one that starts at a multiple of
+ * B2O_STATE_BLOCK and ends at one or at the larger tensor's end (every pointer
+ * at the slice's first element or block): the result is then that of the whole. */
+typedef struct {
+  void* param;             /* param_dtype, numel elements                 */
+  uint16_t* rem;           /* bf16 remainder of a bf16 weight, or NULL    */
+  const void* grad;        /* param_dtype                                 */
+  int8_t* exp_avg;         /* SIGNED codes                                */
+  uint8_t* exp_avg_sq;     /* ROOT codes                                  */
+  float* exp_avg_scale;    /* b2o_state_blocks(numel) each                */
+  float* exp_avg_sq_scale;
+  float* ema;              /* fp32 EMA shadow or NULL                     */
+  int64_t numel;
+  int64_t first;           /* slice of a larger tensor: index of its first element there, else 0 */
+  int32_t group;           /* index into the group table                  */
+  int32_t _pad;
+  float* step_out;         /* 0-d fp32 step tensor the pass sets, or NULL */
+} b2o_adamw8_tensor;
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  double step;             /* step count after increment, >= 1; the t of the codes */
+  const float* grad_scale; /* as in b2o_adamw_group                       */
+  int32_t cautious;
+  int32_t _pad;
+} b2o_adamw8_group;
+int b2o_adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8_group* groups, int ngroups,
+                    int param_dtype, float ema_weight, void* stream);
+
 /* Stand-alone EMA: shadow = lerp(shadow, float(param), weight) for each tensor.
  * Replaces EmaWeights.update/_update_slow (transformer_lm/sol_modules.py:1255-1268). */
 int b2o_ema_update(float* const* shadows, const void* const* params, const int64_t* numels,
@@ -226,6 +292,19 @@ int b2o_normuon_front_multi(const b2o_normuon_batch* batches, int nbatches, int 
  * as for the front call that preceded it. */
 int b2o_normuon_prescale(const b2o_normuon_batch* batches, int nbatches, int dtype, float w_small, float w_large,
                          int nesterov, const float* d_grad_scale, float norm_eps, float norm_safety, void* stream);
+/* The front and prescale calls with the momentum in 8 bits (SIGNED, see
+ * b2o_state_tensor): bufs hold S pointers to int8 codes per batch,
+ * buf_scales[k][s] the fp32 scales of matrix s of batch k
+ * (b2o_state_blocks(r * c) each) and buf_steps[k][s] (host memory) its step
+ * count, the t of the codes. momentum = beta * momentum + (1 - beta) * g;
+ * u is taken from the momentum as it is stored, so the prescale call's rewrite
+ * of X0 gives what the front would have written. */
+int b2o_normuon_front8_multi(const b2o_normuon_batch* batches, float* const* const* buf_scales,
+                             const uint32_t* const* buf_steps, int nbatches, int dtype, double beta, int nesterov,
+                             const float* d_grad_scale, void* stream);
+int b2o_normuon_prescale8(const b2o_normuon_batch* batches, float* const* const* buf_scales, int nbatches, int dtype,
+                          double beta, int nesterov, const float* d_grad_scale, float norm_eps, float norm_safety,
+                          void* stream);
 int b2o_normuon_apply_multi(const b2o_normuon_batch* batches, int nbatches, int param_dtype, float neg_lr,
                             float lr_wd, float wd_factor, int wd_on, int cautious, float w_beta2,
                             float ema_weight, void* stream);
