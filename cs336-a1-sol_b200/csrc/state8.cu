@@ -7,7 +7,6 @@
 #include "b2o_common.cuh"
 #include "b2o_internal.h"
 #include "state8.cuh"
-#include "vec_io.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -16,33 +15,14 @@
 
 namespace b2o {
 
+static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 constexpr int kS8Threads = 256;
 constexpr int kS8Tensors = 96;
 constexpr int kS8Groups = 8;
 constexpr int kS8Chunk = (kS8Threads / 32) * kQ8Tile * 4;  // elements per CTA step: four tiles a warp
 
 static inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
-
-// Eight elements at p + i of a list that ends at `end`; elements behind it read as 0.
-template <typename T>
-__device__ __forceinline__ void load_some(const T* p, int64_t i, int64_t end, bool vec, float* x) {
-  if (vec) {
-    Elem<T>::load8(p + i, x);
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) x[k] = i + k < end ? Elem<T>::load1(p + i + k) : 0.0f;
-}
-template <typename T>
-__device__ __forceinline__ void store_some(T* p, int64_t i, int64_t end, bool vec, const float* x) {
-  if (vec) {
-    Elem<T>::store8(p + i, x);
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (i + k < end) Elem<T>::store1(p + i + k, x[k]);
-}
 
 // ================================================================ AdamW ===
 // Coefficients of one group: bias corrections and 1 - beta from double on the
@@ -53,7 +33,11 @@ struct Adam8Coef {
   float lr_wd;
   float step;                     // torch's state["step"]
   uint32_t turn;                  // the step count that the codes' offsets run with
+  float one;                      // 1 (see mul_add2)
   int wd_on, cautious;
+  // 1: roots of subnormal second moments may read as 0 in the update (eps
+  // covers them by 2^24 times); 0: they are computed (a few instructions more)
+  int plain_roots;
   const float* grad_scale;
 };
 
@@ -76,89 +60,154 @@ __device__ __forceinline__ int find_tensor(const Table& tab, int chunk) {
   return lo;
 }
 
+// One warp step: 256 elements, 8 a lane, blocks of 16 lanes.
+// FULL: all of them exist and every pointer takes vector accesses; EXTRA: the
+// group may have a clip coefficient, weight decay or an eps that does not cover
+// subnormal roots.
+// `mine` are the step's first inputs, loaded during the step before.
 template <typename PT>
-__global__ void __launch_bounds__(kS8Threads) adamw8_kernel(const __grid_constant__ Adam8Table tab) {
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int total = tab.chunk_start[tab.ntensors];
-  for (int chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
-    const int ti = find_tensor(tab, chunk);
-    const b2o_adamw8_tensor& T = tab.t[ti];
-    const Adam8Coef& c = tab.g[T.group];
-    if (T.step_out && chunk == tab.chunk_start[ti] && threadIdx.x == 0) *T.step_out = c.step;
-    const int64_t base = static_cast<int64_t>(chunk - tab.chunk_start[ti]) * kS8Chunk;
-    const int64_t end = min(T.numel, base + kS8Chunk);
-    PT* __restrict__ P = static_cast<PT*>(T.param);
-    const PT* __restrict__ G = static_cast<const PT*>(T.grad);
-    const bool aligned = tab.vec_ok[ti] != 0;
-    const float gs = c.grad_scale ? *c.grad_scale : 1.0f;
-    for (int64_t tile = base + (threadIdx.x >> 5) * kQ8Tile; tile < end; tile += (kS8Threads / 32) * kQ8Tile) {
-      const int64_t i = tile + lane * 8;
-      const bool vec = aligned && i + 8 <= end;
-      const int64_t blk = i / kQ8Block;
-      float g[8], w[8], m[8], v[8];
-      load_some(G, i, end, vec, g);
-      load_some(P, i, end, vec, w);
-      const float ms = i < end ? T.exp_avg_scale[blk] : 0.0f;
-      const float vs = i < end ? T.exp_avg_sq_scale[blk] : 0.0f;
-      unpack_signed(load_codes(T.exp_avg, i, end, vec), ms, m);
-      unpack_root(load_codes(T.exp_avg_sq, i, end, vec), vs, v);
-      if (T.rem) {
-        float r[8];
-        load_some(T.rem, i, end, vec, r);
+struct Adam8In {
+  Raw8<PT> g;
+  uint2 mc, vc;
+  float ms, vs;
+  __device__ __forceinline__ void load(const b2o_adamw8_tensor& T, int64_t i, int64_t end, bool vec, bool in) {
+    g.load(static_cast<const PT*>(T.grad), i, end, vec);
+    mc = load_codes(T.exp_avg, i, end, vec);
+    vc = load_codes(T.exp_avg_sq, i, end, vec);
+    ms = in ? T.exp_avg_scale[i / kQ8Block] : 0.0f;
+    vs = in ? T.exp_avg_sq_scale[i / kQ8Block] : 0.0f;
+  }
+};
+
+template <typename PT, bool REM, bool EMA, bool EXTRA, bool FULL>
+__device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Adam8Coef& c, float ema_weight,
+                                            const Adam8In<PT>& mine, int64_t i, int64_t end, bool aligned, float gs) {
+  const bool vec = FULL || (aligned && i + 8 <= end);
+  const bool in = FULL || i < end;
+  const int64_t blk = i / kQ8Block;
+  PT* const P = static_cast<PT*>(T.param);
+  Raw8<PT> graw = mine.g, praw;
+  Raw8<uint16_t> rraw;
+  Raw8<float> eraw;
+  praw.load(P, i, end, vec);
+  if (REM) rraw.load(T.rem, i, end, vec);
+  if (EMA) eraw.load(T.ema, i, end, vec);
+  V8 g = graw.get();
+  if (EXTRA && c.grad_scale) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] += r[k];
-      }
-      if (c.grad_scale) {
+    for (int j = 0; j < 4; ++j) g.p[j] = mul2(g.p[j], f2(gs));
+    graw.set(g);  // clipped gradient g = dtype(g * coef)
+    g = graw.get();
+  }
+  // Each product and sum of the moments rounds by itself: what is stored
+  // depends on their fp32 values alone, whatever the compiler contracts.
+  V8 m = unpack_signed(mine.mc, mine.ms), v = unpack_root(mine.vc, mine.vs);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g[k] = Elem<PT>::rnd(g[k] * gs);
-      }
-      // Each product and sum of the moments rounds by itself: what is stored
-      // depends on their fp32 values alone, whatever the compiler contracts.
+  for (int j = 0; j < 4; ++j) {
+    m.p[j] = mul_add2(f2(c.b1), m.p[j], mul2(f2(c.w1), g.p[j]), c.one);
+    v.p[j] = mul_add2(f2(c.b2), v.p[j], mul2(f2(c.w2), mul2(g.p[j], g.p[j])), c.one);
+  }
+  const BlockScale sm = signed_scale(block_max(m));
+  const BlockScale sv = root_scale(block_max(v));
+  V8 r;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        m[k] = __fadd_rn(__fmul_rn(c.b1, m[k]), __fmul_rn(c.w1, g[k]));
-        v[k] = __fadd_rn(__fmul_rn(c.b2, v[k]), __fmul_rn(c.w2, __fmul_rn(g[k], g[k])));
-      }
-      const BlockScale sm = signed_scale(block_max(max_abs_bits(m)));
-      const BlockScale sv = root_scale(block_max(max_abs_bits(v)));
-      float r[8];
+  for (int j = 0; j < 4; ++j) {
+    const float2 x = f2_split(v.p[j]);
+    if (!EXTRA || c.plain_roots) r.p[j] = f2(sqrt_approx_ftz(x.x), sqrt_approx_ftz(x.y));
+    else r.p[j] = f2(sqrt_approx(x.x), sqrt_approx(x.y));
+  }
+  if (!in) return;
+  V8 w = praw.get();
+  if (REM) {
+    const V8 q = rraw.get();
 #pragma unroll
-      for (int k = 0; k < 8; ++k) r[k] = sqrt_approx(v[k]);
-      const uint32_t h = dither_of(T.first + i, c.turn);
-      if (i < end) {
-        store_codes(T.exp_avg, i, end, vec, pack_signed<true>(m, sm, h));
-        store_codes(T.exp_avg_sq, i, end, vec, pack_root<true>(v, r, sv, h));
-        if ((lane & 15) == 0) {
-          T.exp_avg_scale[blk] = sm.s;
-          T.exp_avg_sq_scale[blk] = sv.s;
-        }
-      }
-      float p[8];
+    for (int j = 0; j < 4; ++j) w.p[j] = add2(w.p[j], q.p[j]);
+  }
+  if (EXTRA && c.wd_on) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (c.wd_on) w[k] -= (!c.cautious || m[k] * w[k] > 0.0f) ? c.lr_wd * w[k] : 0.0f;
-        w[k] -= __fdividef(c.step_size * m[k], fmaf(r[k], c.inv_bc2, c.eps));
-        p[k] = Elem<PT>::rnd(w[k]);
-      }
-      if (i < end) {
-        store_some(P, i, end, vec, p);
-        if (T.rem) {
-          float q[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) q[k] = w[k] - p[k];
-          store_some(T.rem, i, end, vec, q);
-        }
-        if (T.ema) {
-          float e[8];
-          load_some(T.ema, i, end, vec, e);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) e[k] = torch_lerp(e[k], p[k], tab.ema_weight);
-          store_some(T.ema, i, end, vec, e);
-        }
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = f2_split(w.p[j]), y = f2_split(m.p[j]);
+      const float kx = !c.cautious || x.x * y.x > 0.0f ? -c.lr_wd : 0.0f;
+      const float ky = !c.cautious || x.y * y.y > 0.0f ? -c.lr_wd : 0.0f;
+      w.p[j] = fma2(w.p[j], f2(kx, ky), w.p[j]);
     }
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 d = f2_split(fma2(r.p[j], f2(c.inv_bc2), f2(c.eps)));
+    w.p[j] = fma2(mul2(m.p[j], f2(-c.step_size)), f2(rcp_approx_ftz(d.x), rcp_approx_ftz(d.y)), w.p[j]);
+  }
+  praw.set(w);
+  praw.store(P, i, end, vec);
+  const V8 p = praw.get();  // the weight as it is stored
+  if (REM) {
+    V8 q;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q.p[j] = fma2(p.p[j], f2(-1.0f), w.p[j]);
+    rraw.set(q);
+    rraw.store(T.rem, i, end, vec);
+  }
+  if (EMA) {
+    V8 e = eraw.get();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = f2_split(e.p[j]), y = f2_split(p.p[j]);
+      e.p[j] = f2(torch_lerp(x.x, y.x, ema_weight), torch_lerp(x.y, y.y, ema_weight));
+    }
+    eraw.set(e);
+    eraw.store(T.ema, i, end, vec);
+  }
+  const uint32_t h = dither_of(T.first + i, c.turn);
+  store_codes(T.exp_avg, i, end, vec, pack_signed<true>(m, sm, h));
+  store_codes(T.exp_avg_sq, i, end, vec, pack_root<true>(v, r, sv, h));
+  if ((threadIdx.x & 15) == 0) {
+    T.exp_avg_scale[blk] = sm.s;
+    T.exp_avg_sq_scale[blk] = sv.s;
+  }
+}
+
+template <typename PT, bool REM, bool EMA, bool EXTRA>
+__global__ void __launch_bounds__(kS8Threads, EMA ? 3 : 4) adamw8_kernel(const __grid_constant__ Adam8Table tab) {
+  pdl_wait();
+  const int ti = find_tensor(tab, blockIdx.x);
+  const b2o_adamw8_tensor& T = tab.t[ti];
+  const Adam8Coef& c = tab.g[T.group];
+  const int first = tab.chunk_start[ti];
+  if (T.step_out && blockIdx.x == first && threadIdx.x == 0) *T.step_out = c.step;
+  const int64_t base = static_cast<int64_t>(blockIdx.x - first) * kS8Chunk;
+  const int64_t end = min(T.numel, base + kS8Chunk);
+  const float gs = EXTRA && c.grad_scale ? *c.grad_scale : 1.0f;
+  const int64_t i0 = base + (threadIdx.x >> 5) * kQ8Tile + (threadIdx.x & 31) * 8;
+  constexpr int kStride = (kS8Threads / 32) * kQ8Tile;
+  // two steps where the registers suffice: fewer moves
+  constexpr int kUnroll = sizeof(PT) == 2 && !EMA && !EXTRA ? 2 : 1;
+  if (tab.vec_ok[ti] && base + kS8Chunk <= T.numel) {
+    Adam8In<PT> next;
+    next.load(T, i0, end, true, true);
+#pragma unroll kUnroll
+    for (int n = 0; n < kS8Chunk / kStride; ++n) {
+      const Adam8In<PT> mine = next;
+      if (n + 1 < kS8Chunk / kStride) next.load(T, i0 + (n + 1) * kStride, end, true, true);
+      adamw8_tile<PT, REM, EMA, EXTRA, true>(T, c, tab.ema_weight, mine, i0 + n * kStride, end, true, gs);
+    }
+  } else {
+#pragma unroll 1
+    for (int64_t i = i0; i - (threadIdx.x & 31) * 8 < end; i += kStride) {
+      Adam8In<PT> mine;
+      mine.load(T, i, end, tab.vec_ok[ti] && i + 8 <= end, i < end);
+      adamw8_tile<PT, REM, EMA, EXTRA, false>(T, c, tab.ema_weight, mine, i, end, tab.vec_ok[ti] != 0, gs);
+    }
+  }
+}
+
+template <typename PT, bool REM>
+static void adamw8_launch(const Adam8Table& tab, int chunks, bool ema, bool extra, cudaStream_t stream) {
+  if (ema)
+    launch_pdl(extra ? adamw8_kernel<PT, REM, true, true> : adamw8_kernel<PT, REM, true, false>, dim3(chunks),
+               dim3(kS8Threads), 0, stream, tab);
+  else
+    launch_pdl(extra ? adamw8_kernel<PT, REM, false, true> : adamw8_kernel<PT, REM, false, false>, dim3(chunks),
+               dim3(kS8Threads), 0, stream, tab);
 }
 
 int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8_group* groups, int ngroups,
@@ -184,8 +233,10 @@ int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8
     c.lr_wd = static_cast<float>(g.lr * g.weight_decay);
     c.step = static_cast<float>(g.step);
     c.turn = static_cast<uint32_t>(static_cast<int64_t>(g.step));
+    c.one = 1.0f;
     c.wd_on = g.weight_decay != 0.0;
     c.cautious = g.cautious;
+    c.plain_roots = c.eps * 5.9604645e-8f >= 1.0842022e-19f * c.inv_bc2;  // eps 2^-24 >= 2^-63 inv_bc2
     c.grad_scale = g.grad_scale;
   }
   tab.ema_weight = ema_weight;
@@ -200,30 +251,36 @@ int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8
     if (t.rem && param_dtype != B2O_BF16) { set_error("adamw8: remainder needs bf16 params"); return -1; }
     if ((t.numel + kS8Chunk - 1) / kS8Chunk > (1ll << 30)) { set_error("adamw8: tensor too large"); return -1; }
   }
-  for (int done = 0; done < ntensors;) {
-    int n = 0, chunks = 0;
-    for (; done + n < ntensors && n < kS8Tensors; ++n) {
-      const b2o_adamw8_tensor& t = tensors[done + n];
-      const int ch = static_cast<int>((t.numel + kS8Chunk - 1) / kS8Chunk);
-      if (n > 0 && chunks + static_cast<int64_t>(ch) > (1ll << 30)) break;
-      tab.t[n] = t;
+  // One launch for each mix of remainder and EMA (one in all, as a rule): the
+  // passes without them are then without their branches too.
+  for (int mix = 0; mix < 4; ++mix) {
+    const bool rem = (mix & 1) != 0, ema = (mix & 2) != 0;
+    for (int at = 0; at < ntensors;) {
+      int n = 0, chunks = 0;
+      bool extra = false;
+      for (; at < ntensors && n < kS8Tensors; ++at) {
+        const b2o_adamw8_tensor& t = tensors[at];
+        if (t.numel == 0 || (t.rem != nullptr) != rem || (t.ema != nullptr) != ema) continue;
+        const int ch = static_cast<int>((t.numel + kS8Chunk - 1) / kS8Chunk);
+        if (n > 0 && chunks + static_cast<int64_t>(ch) > (1ll << 30)) break;
+        tab.t[n] = t;
+        tab.chunk_start[n] = chunks;
+        tab.vec_ok[n] = aligned16(t.param) && aligned16(t.grad) && aligned8(t.exp_avg) && aligned8(t.exp_avg_sq) &&
+                        (!t.rem || aligned16(t.rem)) && (!t.ema || aligned16(t.ema));
+        const Adam8Coef& c = tab.g[t.group];
+        extra = extra || c.grad_scale || c.wd_on || !c.plain_roots;
+        chunks += ch;
+        ++n;
+      }
+      if (n == 0) break;
       tab.chunk_start[n] = chunks;
-      tab.vec_ok[n] = aligned16(t.param) && aligned16(t.grad) && aligned8(t.exp_avg) && aligned8(t.exp_avg_sq) &&
-                      (!t.rem || aligned16(t.rem)) && (!t.ema || aligned16(t.ema));
-      chunks += ch;
-    }
-    tab.chunk_start[n] = chunks;
-    tab.ntensors = n;
-    if (chunks > 0) {
-      const int grid = std::min(chunks, num_sms() * 8);
-      if (param_dtype == B2O_F32)
-        launch_pdl(adamw8_kernel<float>, dim3(grid), dim3(kS8Threads), 0, stream, tab);
-      else
-        launch_pdl(adamw8_kernel<uint16_t>, dim3(grid), dim3(kS8Threads), 0, stream, tab);
+      tab.ntensors = n;
+      if (param_dtype == B2O_F32) adamw8_launch<float, false>(tab, chunks, ema, extra, stream);
+      else if (rem) adamw8_launch<uint16_t, true>(tab, chunks, ema, extra, stream);
+      else adamw8_launch<uint16_t, false>(tab, chunks, ema, extra, stream);
       count_launch();
       if (int e = check_launch("adamw8")) return e;
     }
-    done += n;
   }
   return 0;
 }
@@ -236,85 +293,204 @@ struct StateTable {
   int ntensors;
 };
 
+// Two tiles a step, loads of both before the work of either.
+constexpr int kS8Two = 2;
+
 template <typename VT>
-__device__ __forceinline__ void encode_tile(const b2o_state_tensor& T, int64_t i, int64_t end, bool vec, int lane) {
-  float x[8];
-  load_some(static_cast<const VT*>(T.value), i, end, vec, x);
-  if (T.kind == B2O_STATE_PAIR) {
-    if (i >= end) return;
-    float r[8];
+__device__ __forceinline__ void encode_tiles(const b2o_state_tensor& T, int64_t tile, int64_t end, bool aligned,
+                                             int lane) {
+  Raw8<VT> raw[kS8Two];
+  int64_t i[kS8Two];
+  bool vec[kS8Two];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float p = round_bf16(x[k]);
-      r[k] = x[k] - p;
-      x[k] = p;
+  for (int n = 0; n < kS8Two; ++n) {
+    i[n] = tile + n * kQ8Tile + lane * 8;
+    vec[n] = aligned && i[n] + 8 <= end;
+    raw[n].load(static_cast<const VT*>(T.value), i[n], end, vec[n]);
+  }
+#pragma unroll
+  for (int n = 0; n < kS8Two; ++n) {
+    V8 x = raw[n].get();
+    if (T.kind == B2O_STATE_PAIR) {
+      if (i[n] >= end) continue;
+      Raw8<uint16_t> p, r;
+      p.set(x);
+      const V8 y = p.get();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x.p[j] = fma2(y.p[j], f2(-1.0f), x.p[j]);
+      r.set(x);
+      p.store(static_cast<uint16_t*>(T.codes), i[n], end, vec[n]);
+      r.store(static_cast<uint16_t*>(T.scales), i[n], end, vec[n]);
+      continue;
     }
-    store_some(static_cast<uint16_t*>(T.codes), i, end, vec, x);
-    store_some(static_cast<uint16_t*>(T.scales), i, end, vec, r);
-    return;
-  }
-  const bool root = T.kind == B2O_STATE_ROOT;
-  BlockScale b;
-  uint2 codes;
-  if (root) {
-    // a second moment is not negative: a negative value counts as one that is not a number
+    BlockScale b;
+    uint2 codes;
+    if (T.kind == B2O_STATE_ROOT) {
+      // a second moment is not negative: a negative value counts as one that is not a number
+      V8 r;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = x[k] < 0.0f ? __uint_as_float(0x7fffffffu) : x[k];
-    b = root_scale(block_max(max_abs_bits(x)));
-    float r[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) r[k] = sqrt_approx(x[k]);
-    codes = pack_root<false>(x, r, b, 0);
-  } else {
-    b = signed_scale(block_max(max_abs_bits(x)));
-    codes = pack_signed<false>(x, b, 0);
+      for (int j = 0; j < 4; ++j) {
+        float2 y = f2_split(x.p[j]);
+        y.x = y.x < 0.0f ? __int_as_float(0x7fffffff) : y.x;
+        y.y = y.y < 0.0f ? __int_as_float(0x7fffffff) : y.y;
+        x.p[j] = f2(y.x, y.y);
+        r.p[j] = f2(sqrt_approx_ftz(y.x), sqrt_approx_ftz(y.y));
+      }
+      b = root_scale(block_max(x));
+      codes = pack_root<false>(x, r, b, 0);
+    } else {
+      b = signed_scale(block_max(x));
+      codes = pack_signed<false>(x, b, 0);
+    }
+    if (i[n] >= end) continue;
+    store_codes(T.codes, i[n], end, vec[n], codes);
+    if ((lane & 15) == 0) static_cast<float*>(T.scales)[i[n] / kQ8Block] = b.s;
   }
-  if (i >= end) return;
-  store_codes(T.codes, i, end, vec, codes);
-  if ((lane & 15) == 0) static_cast<float*>(T.scales)[i / kQ8Block] = b.s;
 }
 
 template <typename VT>
-__device__ __forceinline__ void decode_tile(const b2o_state_tensor& T, int64_t i, int64_t end, bool vec) {
-  if (i >= end) return;
-  float x[8];
-  if (T.kind == B2O_STATE_PAIR) {
-    float r[8];
-    load_some(static_cast<const uint16_t*>(T.codes), i, end, vec, x);
-    load_some(static_cast<const uint16_t*>(T.scales), i, end, vec, r);
+__device__ __forceinline__ void decode_tiles(const b2o_state_tensor& T, int64_t tile, int64_t end, bool aligned,
+                                             int lane) {
+  int64_t i[kS8Two];
+  bool vec[kS8Two];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] += r[k];
-  } else {
-    const float s = static_cast<const float*>(T.scales)[i / kQ8Block];
-    const uint2 codes = load_codes(T.codes, i, end, vec);
-    if (T.kind == B2O_STATE_ROOT) unpack_root(codes, s, x);
-    else unpack_signed(codes, s, x);
+  for (int n = 0; n < kS8Two; ++n) {
+    i[n] = tile + n * kQ8Tile + lane * 8;
+    vec[n] = aligned && i[n] + 8 <= end;
   }
-  store_some(static_cast<VT*>(T.value), i, end, vec, x);
+  V8 x[kS8Two];
+  if (T.kind == B2O_STATE_PAIR) {
+    Raw8<uint16_t> p[kS8Two], r[kS8Two];
+#pragma unroll
+    for (int n = 0; n < kS8Two; ++n) {
+      p[n].load(static_cast<const uint16_t*>(T.codes), i[n], end, vec[n]);
+      r[n].load(static_cast<const uint16_t*>(T.scales), i[n], end, vec[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < kS8Two; ++n) {
+      x[n] = p[n].get();
+      const V8 y = r[n].get();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[n].p[j] = add2(x[n].p[j], y.p[j]);
+    }
+  } else {
+    float s[kS8Two];
+    uint2 codes[kS8Two];
+#pragma unroll
+    for (int n = 0; n < kS8Two; ++n) {
+      codes[n] = load_codes(T.codes, i[n], end, vec[n]);
+      s[n] = i[n] < end ? static_cast<const float*>(T.scales)[i[n] / kQ8Block] : 0.0f;
+    }
+#pragma unroll
+    for (int n = 0; n < kS8Two; ++n)
+      x[n] = T.kind == B2O_STATE_ROOT ? unpack_root(codes[n], s[n]) : unpack_signed(codes[n], s[n]);
+  }
+#pragma unroll
+  for (int n = 0; n < kS8Two; ++n) {
+    if (i[n] >= end) continue;
+    Raw8<VT> raw;
+    raw.set(x[n]);
+    raw.store(static_cast<VT*>(T.value), i[n], end, vec[n]);
+  }
+}
+
+// A whole chunk decoded, vector accesses: a warp takes 1024 elements in a row.
+// fp32 values are written 4 a lane, so that a store covers 512 bytes in a row:
+// with 8 a lane, in two halves 32 bytes apart, 33.5 M codes took 37 us instead
+// of 26. Stores are streaming ones: nothing here reads them again.
+constexpr int kS8Warp = kS8Chunk / (kS8Threads / 32);
+
+__device__ __forceinline__ void decode_whole(const b2o_state_tensor& T, int64_t at, int lane, float) {
+  constexpr int kN = kS8Warp / kQ8Block;
+  float* const out = static_cast<float*>(T.value) + at + lane * 4;
+  if (T.kind == B2O_STATE_PAIR) {
+    uint2 p[kN], r[kN];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      p[n] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(T.codes) + at + n * kQ8Block + lane * 4);
+      r[n] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(T.scales) + at + n * kQ8Block + lane * 4);
+    }
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const float2 x = f2_split(add2(Raw8<uint16_t>::pair(p[n].x), Raw8<uint16_t>::pair(r[n].x)));
+      const float2 y = f2_split(add2(Raw8<uint16_t>::pair(p[n].y), Raw8<uint16_t>::pair(r[n].y)));
+      __stcs(reinterpret_cast<float4*>(out + n * kQ8Block), make_float4(x.x, x.y, y.x, y.y));
+    }
+    return;
+  }
+  const float* const sc = static_cast<const float*>(T.scales) + at / kQ8Block;
+  uint32_t w[kN];
+  float s[kN];
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+    w[n] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(T.codes) + at + n * kQ8Block + lane * 4);
+    s[n] = sc[n];
+  }
+  const bool root = T.kind == B2O_STATE_ROOT;
+#pragma unroll
+  for (int n = 0; n < kN; ++n) __stcs(reinterpret_cast<float4*>(out + n * kQ8Block), unpack4(w[n], s[n], root));
+}
+
+__device__ __forceinline__ void decode_whole(const b2o_state_tensor& T, int64_t at, int lane, uint16_t) {
+  constexpr int kN = kS8Warp / kQ8Tile;
+  const int64_t i = at + lane * 8;
+  uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(T.value) + i);
+  if (T.kind == B2O_STATE_PAIR) {
+    Raw8<uint16_t> p[kN], r[kN];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      p[n].load(static_cast<const uint16_t*>(T.codes), i + n * kQ8Tile, 0, true);
+      r[n].load(static_cast<const uint16_t*>(T.scales), i + n * kQ8Tile, 0, true);
+    }
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      V8 x = p[n].get();
+      const V8 y = r[n].get();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x.p[j] = add2(x.p[j], y.p[j]);
+      p[n].set(x);
+      __stcs(out + n * (kQ8Tile / 8), p[n].a);
+    }
+    return;
+  }
+  uint2 w[kN];
+  float s[kN];
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+    w[n] = load_codes(T.codes, i + n * kQ8Tile, 0, true);
+    s[n] = static_cast<const float*>(T.scales)[i / kQ8Block + 2 * n];
+  }
+  const bool root = T.kind == B2O_STATE_ROOT;
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+    Raw8<uint16_t> v;
+    v.set(root ? unpack_root(w[n], s[n]) : unpack_signed(w[n], s[n]));
+    __stcs(out + n * (kQ8Tile / 8), v.a);
+  }
+}
+
+template <bool ENCODE, typename VT>
+__device__ __forceinline__ void state_chunk(const b2o_state_tensor& T, int64_t base, bool aligned) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t end = min(T.numel, base + kS8Chunk);
+  if (!ENCODE && aligned && base + kS8Chunk <= T.numel) {
+    decode_whole(T, base + warp * kS8Warp, lane, VT());
+    return;
+  }
+  for (int64_t tile = base + warp * (kS8Two * kQ8Tile); tile < end; tile += (kS8Threads / 32) * (kS8Two * kQ8Tile)) {
+    if (ENCODE) encode_tiles<VT>(T, tile, end, aligned, lane);
+    else decode_tiles<VT>(T, tile, end, aligned, lane);
+  }
 }
 
 template <bool ENCODE>
 __global__ void __launch_bounds__(kS8Threads) state_kernel(const __grid_constant__ StateTable tab) {
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int total = tab.chunk_start[tab.ntensors];
-  for (int chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
-    const int ti = find_tensor(tab, chunk);
-    const b2o_state_tensor& T = tab.t[ti];
-    const int64_t base = static_cast<int64_t>(chunk - tab.chunk_start[ti]) * kS8Chunk;
-    const int64_t end = min(T.numel, base + kS8Chunk);
-    for (int64_t tile = base + (threadIdx.x >> 5) * kQ8Tile; tile < end; tile += (kS8Threads / 32) * kQ8Tile) {
-      const int64_t i = tile + lane * 8;
-      const bool vec = tab.vec_ok[ti] && i + 8 <= end;
-      if (T.value_dtype == B2O_F32) {
-        if (ENCODE) encode_tile<float>(T, i, end, vec, lane);
-        else decode_tile<float>(T, i, end, vec);
-      } else {
-        if (ENCODE) encode_tile<uint16_t>(T, i, end, vec, lane);
-        else decode_tile<uint16_t>(T, i, end, vec);
-      }
-    }
-  }
+  const int ti = find_tensor(tab, blockIdx.x);
+  const b2o_state_tensor& T = tab.t[ti];
+  const int64_t base = static_cast<int64_t>(blockIdx.x - tab.chunk_start[ti]) * kS8Chunk;
+  if (T.value_dtype == B2O_F32) state_chunk<ENCODE, float>(T, base, tab.vec_ok[ti] != 0);
+  else state_chunk<ENCODE, uint16_t>(T, base, tab.vec_ok[ti] != 0);
 }
 
 template <bool ENCODE>
@@ -351,8 +527,7 @@ static int state_launch(const b2o_state_tensor* tensors, int ntensors, cudaStrea
     tab.chunk_start[n] = chunks;
     tab.ntensors = n;
     if (chunks > 0) {
-      const int grid = std::min(chunks, num_sms() * 8);
-      launch_pdl(state_kernel<ENCODE>, dim3(grid), dim3(kS8Threads), 0, stream, tab);
+      launch_pdl(state_kernel<ENCODE>, dim3(chunks), dim3(kS8Threads), 0, stream, tab);
       count_launch();
       if (int e = check_launch(what.c_str())) return e;
     }

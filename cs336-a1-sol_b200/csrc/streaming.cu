@@ -663,8 +663,77 @@ struct Front8Table {
   const float* gscale;
 };
 
-template <typename T, bool REPAIR>
-__device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, float beta, float w1, int nesterov) {
+// What a warp step reads: loaded during the step before.
+template <typename T>
+struct Front8In {
+  Raw8<T> g;
+  uint2 codes;
+  float s;
+  __device__ __forceinline__ void load(const T* G, const void* B, const float* SC, int64_t i, int64_t end, bool vec,
+                                       bool in) {
+    g.load(G, i, end, vec);
+    codes = load_codes(B, i, end, vec);
+    s = in ? SC[i / kQ8Block] : 0.0f;
+  }
+};
+struct Front8Args {
+  float beta, w1, one, kx, gs;
+  int x0;
+  uint32_t step;
+};
+
+// One warp step: 256 elements, 8 a lane. FULL: all exist, vector accesses.
+template <typename T, bool REPAIR, bool NESTEROV, bool CLIP, bool FULL>
+__device__ __forceinline__ void front8_tile(const Front8In<T>& in8, const Front8Args& a, void* B, float* SC, uint16_t* U,
+                                            int64_t i, int64_t end, bool aligned, F2& acc) {
+  const bool vec = FULL || (aligned && i + 8 <= end);
+  const bool in = FULL || i < end;
+  Raw8<T> graw = in8.g;
+  V8 g = graw.get();
+  if (CLIP) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g.p[j] = mul2(g.p[j], f2(a.gs));
+    graw.set(g);
+    g = graw.get();
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) g.p[j] = mul2(f2(a.w1), g.p[j]);
+  V8 m = unpack_signed(in8.codes, in8.s);
+  if (!REPAIR) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m.p[j] = mul_add2(f2(a.beta), m.p[j], g.p[j], a.one);
+    const BlockScale b = signed_scale(block_max(m));
+    const uint2 codes = pack_signed<true>(m, b, dither_of(i, a.step));
+    if (in) {
+      store_codes(B, i, end, vec, codes);
+      if ((threadIdx.x & 15) == 0) SC[i / kQ8Block] = b.s;
+    }
+    m = unpack_signed(codes, b.s);
+  }
+  if (NESTEROV) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m.p[j] = mul_add2(f2(a.beta), m.p[j], g.p[j], a.one);
+  }
+  Raw8<uint16_t> u;
+  u.set(m);
+  if (!in) return;  // (the warp's last step)
+  m = u.get();      // u as bf16 values
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc = fma2(m.p[j], m.p[j], acc);  // elements behind the end are 0
+  if (a.x0) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = f2_split(mul2(m.p[j], f2(a.kx)));
+      w[j] = f32_to_f16(x.x) | static_cast<uint32_t>(f32_to_f16(x.y)) << 16;
+    }
+    u.a = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  u.store(U, i, end, vec);
+}
+
+template <typename T, bool REPAIR, bool NESTEROV, bool CLIP>
+__device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, float beta, float w1, float one) {
   const MultiBatchInfo& bi = tab.h.b[find_batch_cta(tab.h, cta)];
   const int local = cta - bi.cta0;
   const int s = local / bi.nparts;
@@ -673,59 +742,40 @@ __device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, flo
   const T* G = static_cast<const T*>(tab.g[bi.mat0 + s]);
   void* B = tab.buf[bi.mat0 + s];
   float* SC = tab.scale[bi.mat0 + s];
-  const uint32_t step = tab.step[bi.mat0 + s];
-  uint16_t* Us = bi.u + static_cast<int64_t>(s) * rc;
-  const bool x0 = bi.x0_half != 0;
-  const float kx = x0 ? bi.prescale[s] : 1.0f;
+  uint16_t* U = bi.u + static_cast<int64_t>(s) * rc;
   const int64_t base = static_cast<int64_t>(part) * kFrontPart;
   const int64_t end = min(rc, base + kFrontPart);
-  const bool clip = tab.gscale != nullptr;
-  const float gs = clip ? *tab.gscale : 1.0f;
+  Front8Args a;
+  a.beta = beta; a.w1 = w1; a.one = one;
+  a.x0 = bi.x0_half != 0;
+  a.kx = a.x0 ? bi.prescale[s] : 1.0f;
+  // clipped gradient g = dtype(g * coef), as torch._foreach_mul_ leaves it
+  a.gs = CLIP ? *tab.gscale : 1.0f;
+  a.step = tab.step[bi.mat0 + s];
   const int lane = threadIdx.x & 31;
-  float pacc = 0.f;
-  for (int64_t tile = base + (threadIdx.x >> 5) * kQ8Tile; tile < end; tile += (kFrontThreads / 32) * kQ8Tile) {
-    const int64_t i = tile + lane * 8;
-    const bool vec = bi.vec_ok && i + 8 <= end;
-    float g[8], m[8];
-    if (vec) {
-      Elem<T>::load8(G + i, g);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) g[k] = i + k < end ? Elem<T>::load1(G + i + k) : 0.0f;
+  F2 acc = f2(0.0f);
+  const int64_t i0 = base + (threadIdx.x >> 5) * kQ8Tile + lane * 8;
+  constexpr int kStride = (kFrontThreads / 32) * kQ8Tile;
+  if (bi.vec_ok && base + kFrontPart <= rc) {
+    Front8In<T> next;
+    next.load(G, B, SC, i0, end, true, true);
+#pragma unroll 2
+    for (int n = 0; n < kFrontPart / kStride; ++n) {
+      const Front8In<T> mine = next;
+      if (n + 1 < kFrontPart / kStride) next.load(G, B, SC, i0 + (n + 1) * kStride, end, true, true);
+      front8_tile<T, REPAIR, NESTEROV, CLIP, true>(mine, a, B, SC, U, i0 + n * kStride, end, true, acc);
     }
-    if (clip) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) g[k] = Elem<T>::rnd(g[k] * gs);
-    }
-    const float sc = i < end ? SC[i / kQ8Block] : 0.0f;
-    uint2 codes = load_codes(B, i, end, vec);
-    unpack_signed(codes, sc, m);
-    if (!REPAIR) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) m[k] = __fadd_rn(__fmul_rn(beta, m[k]), __fmul_rn(w1, g[k]));
-      const BlockScale b = signed_scale(block_max(max_abs_bits(m)));
-      codes = pack_signed<true>(m, b, dither_of(i, step));
-      if (i < end) {
-        store_codes(B, i, end, vec, codes);
-        if ((lane & 15) == 0) SC[i / kQ8Block] = b.s;
-      }
-      unpack_signed(codes, b.s, m);
-    }
-    float u[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      u[k] = round_bf16(nesterov ? __fadd_rn(__fmul_rn(beta, m[k]), __fmul_rn(w1, g[k])) : m[k]);
-      if (i + k < end) pacc = fmaf(u[k], u[k], pacc);
-    }
-    if (vec) {
-      store_u8(Us + i, u, x0, kx);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (i + k < end) Us[i + k] = x0 ? f32_to_f16(u[k] * kx) : f32_to_bf16(u[k]);
+  } else {
+#pragma unroll 1
+    for (int64_t i = i0; i - lane * 8 < end; i += kStride) {
+      Front8In<T> mine;
+      mine.load(G, B, SC, i, end, bi.vec_ok && i + 8 <= end, i < end);
+      front8_tile<T, REPAIR, NESTEROV, CLIP, false>(mine, a, B, SC, U, i, end, bi.vec_ok != 0, acc);
     }
   }
   if (REPAIR) return;
+  const float2 halves = f2_split(acc);
+  float pacc = halves.x + halves.y;
   // fixed-order block reduction of this part
   __shared__ float red[kFrontThreads / 32];
 #pragma unroll
@@ -739,16 +789,16 @@ __device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, flo
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kFrontThreads) normuon_front8_kernel(const __grid_constant__ Front8Table tab,
-                                                                       float beta, float w1, int nesterov) {
+template <typename T, bool NESTEROV, bool CLIP>
+__global__ void __launch_bounds__(kFrontThreads, CLIP ? 4 : 5) normuon_front8_kernel(const __grid_constant__ Front8Table tab,
+                                                                          float beta, float w1, float one) {
   pdl_wait();
-  front8_body<T, false>(tab, blockIdx.x, beta, w1, nesterov);
+  front8_body<T, false, NESTEROV, CLIP>(tab, blockIdx.x, beta, w1, one);
 }
 
-template <typename T>
+template <typename T, bool NESTEROV, bool CLIP>
 __global__ void __launch_bounds__(kFrontThreads) normuon_x0_repair8_kernel(const __grid_constant__ Front8Table tab,
-                                                                           float beta, float w1, int nesterov) {
+                                                                           float beta, float w1, float one) {
   pdl_wait();
   const int m = blockIdx.x / kRepairCtas;
   const int sub = blockIdx.x - m * kRepairCtas;
@@ -758,7 +808,19 @@ __global__ void __launch_bounds__(kFrontThreads) normuon_x0_repair8_kernel(const
   const int s = m - bi.mat0;
   if (!bi.x0_half || !bi.flags[s]) return;
   for (int part = sub; part < bi.nparts; part += kRepairCtas)
-    front8_body<T, true>(tab, bi.cta0 + s * bi.nparts + part, beta, w1, nesterov);
+    front8_body<T, true, NESTEROV, CLIP>(tab, bi.cta0 + s * bi.nparts + part, beta, w1, one);
+}
+
+template <typename T>
+static void front8_enqueue(const Front8Table& tab, int grid, float beta, float w1, int nesterov, bool repair,
+                           cudaStream_t stream) {
+  const bool clip = tab.gscale != nullptr;
+  auto front = nesterov ? (clip ? normuon_front8_kernel<T, true, true> : normuon_front8_kernel<T, true, false>)
+                        : (clip ? normuon_front8_kernel<T, false, true> : normuon_front8_kernel<T, false, false>);
+  auto fix = nesterov ? (clip ? normuon_x0_repair8_kernel<T, true, true> : normuon_x0_repair8_kernel<T, true, false>)
+                      : (clip ? normuon_x0_repair8_kernel<T, false, true> : normuon_x0_repair8_kernel<T, false, false>);
+  launch_pdl(repair ? fix : front, dim3(grid), dim3(kFrontThreads), 0, stream, tab, beta, w1, 1.0f);
+  count_launch();
 }
 
 static int front8_launch(const b2o_normuon_batch* batches, float* const* const* buf_scales,
@@ -781,23 +843,14 @@ static int front8_launch(const b2o_normuon_batch* batches, float* const* const* 
     }
   }
   const float b = static_cast<float>(beta), w1 = static_cast<float>(1.0 - beta);
+  int grid = ncta;
   if (repair) {
     if (int e = prescale_launch(tab.h, nmats, norm_eps, norm_safety, stream)) return e;
-    const int rgrid = nmats * kRepairCtas;
-    if (dtype == B2O_F32)
-      launch_pdl(normuon_x0_repair8_kernel<float>, dim3(rgrid), dim3(kFrontThreads), 0, stream, tab, b, w1, nesterov);
-    else
-      launch_pdl(normuon_x0_repair8_kernel<uint16_t>, dim3(rgrid), dim3(kFrontThreads), 0, stream, tab, b, w1,
-                 nesterov);
-    count_launch();
-    return check_launch("normuon_x0_repair8");
+    grid = nmats * kRepairCtas;
   }
-  if (dtype == B2O_F32)
-    launch_pdl(normuon_front8_kernel<float>, dim3(ncta), dim3(kFrontThreads), 0, stream, tab, b, w1, nesterov);
-  else
-    launch_pdl(normuon_front8_kernel<uint16_t>, dim3(ncta), dim3(kFrontThreads), 0, stream, tab, b, w1, nesterov);
-  count_launch();
-  return check_launch("normuon_front8");
+  if (dtype == B2O_F32) front8_enqueue<float>(tab, grid, b, w1, nesterov, repair, stream);
+  else front8_enqueue<uint16_t>(tab, grid, b, w1, nesterov, repair, stream);
+  return check_launch(repair ? "normuon_x0_repair8" : "normuon_front8");
 }
 
 int normuon_front8_multi(const b2o_normuon_batch* batches, float* const* const* buf_scales,
