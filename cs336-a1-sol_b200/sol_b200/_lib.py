@@ -250,7 +250,14 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
                            "there is no CPU fallback")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: torch.device | None = None) -> int:
+    """The current stream of a device (the current device's by default)."""
+    if _raw_stream is not None and torch.cuda.is_initialized():
+        index = device.index if device is not None else None
+        return _raw_stream(torch.cuda.current_device() if index is None else index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

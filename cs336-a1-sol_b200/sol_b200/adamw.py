@@ -160,24 +160,34 @@ class AdamW(torch.optim.Optimizer):
         moments are those of its own rows until ``gather_state``.)"""
         if params is None:
             params = [p for g in self.param_groups for p in g["params"]]
-        items, dts, out, where = [], [], [], []
-        for i, p in enumerate(params):
-            _lib.require_cuda(p, "AdamW.expanded_state")
-            st = self._init_state(p)
-            out.append({})
-            if st["exp_avg"].dtype == torch.int8:
-                items += [(st["exp_avg"], st["exp_avg_scale"], "signed"), (st["exp_avg_sq"], st["exp_avg_sq_scale"], "root")]
-                dts += [dtype, dtype]
-                where += [(i, "exp_avg"), (i, "exp_avg_sq")]
+        value_code = state8._VALUE_CODE.get(dtype)
+        if value_code is None:
+            raise TypeError(f"AdamW.expanded_state: float32 or bfloat16 (got {dtype})")
+        out, rows, eight, empty = [], state8.Rows(), torch.int8, torch.empty_like
+        for p in params:
+            if not p.is_cuda:
+                _lib.require_cuda(p, "AdamW.expanded_state")
+            st = self.state.get(p)
+            if not st or "exp_avg" not in st:
+                st = self._init_state(p)
+            m, v, n = st["exp_avg"], st["exp_avg_sq"], p.numel()
+            wide = {}
+            if m.dtype == eight:
+                wide["exp_avg"], wide["exp_avg_sq"] = a, b = empty(m, dtype=dtype), empty(v, dtype=dtype)
+                if n:
+                    rows.add(a, m, st["exp_avg_scale"], n, 0, value_code)
+                    rows.add(b, v, st["exp_avg_sq_scale"], n, 1, value_code)
             else:
-                out[i]["exp_avg"] = st["exp_avg"].to(dtype, copy=True)
-                out[i]["exp_avg_sq"] = st["exp_avg_sq"].to(dtype, copy=True)
-            if "mant_rem" in st:
-                items.append((p.detach(), st["mant_rem"], "pair"))
-                dts.append(torch.float32)
-                where.append((i, "master"))
-        for (i, key), v in zip(where, state8.decode(items, dtype=dts)):
-            out[i][key] = v
+                wide["exp_avg"], wide["exp_avg_sq"] = m.to(dtype, copy=True), v.to(dtype, copy=True)
+            rem = st.get("mant_rem")
+            if rem is not None:
+                if not p.is_contiguous():
+                    raise ValueError("AdamW.expanded_state: contiguous parameters only")
+                wide["master"] = w = empty(rem, dtype=torch.float32)
+                if n:
+                    rows.add(w, p, rem, n, 2, _lib.F32)
+            out.append(wide)
+        rows.launch(_lib.load().b2o_state_decode, "state_decode")
         return out
 
     def expanded_state_dict(self):
@@ -276,6 +286,20 @@ class AdamW(torch.optim.Optimizer):
                 "keep": ps, "launches": launches, "refresh": refresh, "groups": by_group,
                 "ema_idx": frozenset(ema_idx)}
 
+    def _groups(self, steps_of, grad_scale):
+        """Group table of the pass with wide moments; a group that does not step keeps a row of zeros."""
+        tab = (_lib.AdamwGroup * max(1, len(self.param_groups)))()
+        for gi, group in enumerate(self.param_groups):
+            if gi not in steps_of:
+                continue
+            b1, b2 = group["betas"]
+            lr, wd = float(group["lr"]), float(group["weight_decay"])
+            # torch's fused kernel multiplies fp32(lr) * fp32(weight_decay)
+            lr_wd = float(C.c_float(float(C.c_float(lr).value) * float(C.c_float(wd).value)).value)
+            tab[gi] = _lib.AdamwGroup(lr, float(b1), float(b2), float(group["eps"]), wd, lr_wd, float(steps_of[gi]),
+                                      int(bool(self.cautious_wd)), grad_scale)
+        return tab
+
     def _groups8(self, steps_of, grad_scale):
         """Group table of the 8-bit pass; a group that does not step gets a neutral row."""
         tab = (_lib.Adamw8Group * max(1, len(self.param_groups)))()
@@ -327,33 +351,20 @@ class AdamW(torch.optim.Optimizer):
             k = self._steps.get(ids[0], 0) + 1
             self._steps.update(dict.fromkeys(ids, k))
             steps_of[gi] = k
-        gtab = []
         gsc = self._grad_scale.data_ptr() if self._grad_scale is not None else None
-        for gi, group in enumerate(self.param_groups):
-            if gi not in steps_of:
-                gtab.append(None)
-                continue
-            b1, b2 = group["betas"]
-            lr, wd = float(group["lr"]), float(group["weight_decay"])
-            # torch's fused kernel multiplies fp32(lr) * fp32(weight_decay)
-            lr_wd = float(C.c_float(float(C.c_float(lr).value) * float(C.c_float(wd).value)).value)
-            gtab.append(_lib.AdamwGroup(lr, float(b1), float(b2), float(group["eps"]), wd, lr_wd,
-                                        float(steps_of[gi]), int(bool(self.cautious_wd)), gsc))
-        groups = (_lib.AdamwGroup * max(1, len(gtab)))()
-        for i, g in enumerate(gtab):
-            if g is not None:
-                groups[i] = g
-        groups8 = None
+        groups = groups8 = None
+        ngroups = len(self.param_groups)
         for arr, n, pdt, sdt, dev in plan["launches"]:
             with _lib.on_device(dev):
                 if sdt is None:
                     if groups8 is None:
                         groups8 = self._groups8(steps_of, gsc)
-                    rc = lib.b2o_adamw8_step(arr, n, groups8, len(gtab), pdt, self._ema_weight, _lib.stream_ptr(dev))
+                    rc = lib.b2o_adamw8_step(arr, n, groups8, ngroups, pdt, self._ema_weight, _lib.stream_ptr(dev))
                     _lib.check(rc, "adamw8_step")
                 else:
-                    rc = lib.b2o_adamw_step(arr, n, groups, len(gtab), pdt, sdt, self._ema_weight,
-                                            _lib.stream_ptr(dev))
+                    if groups is None:
+                        groups = self._groups(steps_of, gsc)
+                    rc = lib.b2o_adamw_step(arr, n, groups, ngroups, pdt, sdt, self._ema_weight, _lib.stream_ptr(dev))
                     _lib.check(rc, "adamw_step")
         if self._ema is not None and plan["ema_idx"]:
             self._ema._folded |= plan["ema_idx"]

@@ -21,11 +21,16 @@ tensors of a device, on that device's current stream.
 """
 from __future__ import annotations
 
+import ctypes as C
+from array import array
+
 import torch
 
 from . import _lib
 
 BLOCK = 128
+_WORDS = C.sizeof(_lib.StateTensor) // 8
+_VALUE_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _KINDS = {"signed": 0, "root": 1, "pair": 2}
 _CODE_DTYPE = {"signed": torch.int8, "root": torch.uint8, "pair": torch.bfloat16}
 
@@ -36,60 +41,75 @@ def blocks(numel: int) -> int:
 
 
 def _kind(kind) -> int:
-    if kind not in _KINDS:
-        raise ValueError(f"state kind must be 'signed', 'root' or 'pair' (got {kind!r})")
-    return _KINDS[kind]
+    try:
+        return _KINDS[kind]
+    except (KeyError, TypeError):
+        raise ValueError(f"state kind must be 'signed', 'root' or 'pair' (got {kind!r})") from None
 
 
-def _check_value(t, what):
-    _lib.require_cuda(t, what)
-    if t.dtype not in (torch.float32, torch.bfloat16):
+def _value_code(t, what) -> int:
+    """Checks a tensor of values; its dtype code."""
+    if not t.is_cuda:
+        _lib.require_cuda(t, what)
+    code = _VALUE_CODE.get(t.dtype)
+    if code is None:
         raise TypeError(f"{what}: values are float32 or bfloat16 (got {t.dtype})")
     if not t.is_contiguous():
         raise ValueError(f"{what}: contiguous tensors only")
+    return code
 
 
-def _check_codes(codes, scales, kind, what):
-    for t in (codes, scales):
-        _lib.require_cuda(t, what)
-        if not t.is_contiguous() or t.device != codes.device:
-            raise ValueError(f"{what}: contiguous codes and scales on one device")
-    n = codes.numel()
+def _check_codes(codes, scales, kind, n, what):
+    if not (codes.is_cuda and scales.is_cuda):
+        _lib.require_cuda(codes, what)
+        _lib.require_cuda(scales, what)
+    if not (codes.is_contiguous() and scales.is_contiguous() and codes.get_device() == scales.get_device()):
+        raise ValueError(f"{what}: contiguous codes and scales on one device")
     want = (torch.bfloat16, n) if kind == "pair" else (torch.float32, blocks(n))
-    if codes.dtype != _CODE_DTYPE[kind] or (scales.dtype, scales.numel()) != want:
+    if codes.dtype != _CODE_DTYPE[kind] or scales.dtype != want[0] or scales.numel() != want[1]:
         raise ValueError(f"{what}: a {kind!r} state of {n} elements has {_CODE_DTYPE[kind]} codes and "
                          f"{want[1]} {want[0]} scales (got {codes.dtype}, {scales.numel()} {scales.dtype})")
 
 
-def _launch(fn, what, rows):
-    """rows: (device, value, codes, scales, kind code); one call per device."""
-    by = {}
-    for dev, value, codes, scales, kind in rows:
-        by.setdefault(dev, []).append((value.data_ptr(), codes.data_ptr(), scales.data_ptr(), value.numel(), kind,
-                                       _lib.dtype_code(value.dtype)))
-    for dev, descs in by.items():
-        arr = (_lib.StateTensor * len(descs))(*descs)
-        with _lib.on_device(dev):
-            _lib.check(fn(arr, len(descs), _lib.stream_ptr(dev)), what)
+class Rows:
+    """Descriptors of one call (b2o_state_tensor as 64-bit words), by device."""
+    __slots__ = ("by",)
+
+    def __init__(self):
+        self.by = {}
+
+    def add(self, value, codes, scales, n, kind, value_code):
+        words = self.by.get(value.get_device())
+        if words is None:
+            words = self.by[value.get_device()] = array("Q")
+        words.extend((value.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, kind | value_code << 32))
+
+    def launch(self, fn, what):
+        for index, words in self.by.items():
+            n = len(words) // _WORDS
+            dev = torch.device("cuda", index)
+            with _lib.on_device(dev):
+                _lib.check(fn((_lib.StateTensor * n).from_buffer(words), n, _lib.stream_ptr(dev)), what)
 
 
 @torch.no_grad()
 def encode(items):
     """[(tensor, kind), ...] -> [(codes, scales), ...] ("pair": (bf16 weight, bf16
     remainder)). ``tensor``: contiguous fp32 or bf16 CUDA tensor; codes keep its shape."""
-    out, rows = [], []
+    out, rows = [], Rows()
     for value, kind in items:
         code = _kind(kind)
-        _check_value(value, "state8.encode")
+        value_code = _value_code(value, "state8.encode")
+        n = value.numel()
         codes = torch.empty_like(value, dtype=_CODE_DTYPE[kind])
         if kind == "pair":
             scales = torch.empty_like(codes)
         else:
-            scales = torch.empty(blocks(value.numel()), dtype=torch.float32, device=value.device)
+            scales = torch.empty(blocks(n), dtype=torch.float32, device=value.device)
         out.append((codes, scales))
-        if value.numel():
-            rows.append((value.device, value, codes, scales, code))
-    _launch(_lib.load().b2o_state_encode, "state_encode", rows)
+        if n:
+            rows.add(value, codes, scales, n, code, value_code)
+    rows.launch(_lib.load().b2o_state_encode, "state_encode")
     return out
 
 
@@ -102,21 +122,27 @@ def decode(items, dtype=torch.float32, out=None):
     items = list(items)
     if out is not None and len(out) != len(items):
         raise ValueError(f"state8.decode: {len(items)} states and {len(out)} outputs")
-    if isinstance(dtype, (list, tuple)) and len(dtype) != len(items):
+    many = isinstance(dtype, (list, tuple))
+    if many and len(dtype) != len(items):
         raise ValueError(f"state8.decode: {len(items)} states and {len(dtype)} dtypes")
-    values, rows = [], []
+    values, rows = [], Rows()
     for i, (codes, scales, kind) in enumerate(items):
         code = _kind(kind)
-        _check_codes(codes, scales, kind, "state8.decode")
+        n = codes.numel()
+        _check_codes(codes, scales, kind, n, "state8.decode")
         if out is not None:
             value = out[i]
+            value_code = _value_code(value, "state8.decode")
+            if value.numel() != n or value.get_device() != codes.get_device():
+                raise ValueError("state8.decode: an output has its codes' size and device")
         else:
-            value = torch.empty_like(codes, dtype=dtype[i] if isinstance(dtype, (list, tuple)) else dtype)
-        _check_value(value, "state8.decode")
-        if value.numel() != codes.numel() or value.device != codes.device:
-            raise ValueError("state8.decode: an output has its codes' size and device")
+            dt = dtype[i] if many else dtype
+            value_code = _VALUE_CODE.get(dt)
+            if value_code is None:
+                raise TypeError(f"state8.decode: values are float32 or bfloat16 (got {dt})")
+            value = torch.empty_like(codes, dtype=dt)
         values.append(value)
-        if value.numel():
-            rows.append((value.device, value, codes, scales, code))
-    _launch(_lib.load().b2o_state_decode, "state_decode", rows)
+        if n:
+            rows.add(value, codes, scales, n, code, value_code)
+    rows.launch(_lib.load().b2o_state_decode, "state_decode")
     return values
