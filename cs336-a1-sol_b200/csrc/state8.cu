@@ -107,8 +107,8 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
     m.p[j] = mul_add2(f2(c.b1), m.p[j], mul2(f2(c.w1), g.p[j]), c.one);
     v.p[j] = mul_add2(f2(c.b2), v.p[j], mul2(f2(c.w2), mul2(g.p[j], g.p[j])), c.one);
   }
-  const BlockScale sm = signed_scale(block_max(m));
-  const BlockScale sv = root_scale(block_max(v));
+  const BlockScale sm = signed_scale(block_max<1>(&m));
+  const BlockScale sv = root_scale(block_max<1>(&v));
   V8 r;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -336,10 +336,10 @@ __device__ __forceinline__ void encode_tiles(const b2o_state_tensor& T, int64_t 
         x.p[j] = f2(y.x, y.y);
         r.p[j] = f2(sqrt_approx_ftz(y.x), sqrt_approx_ftz(y.y));
       }
-      b = root_scale(block_max(x));
+      b = root_scale(block_max<1>(&x));
       codes = pack_root<false>(x, r, b, 0);
     } else {
-      b = signed_scale(block_max(x));
+      b = signed_scale(block_max<1>(&x));
       codes = pack_signed<false>(x, b, 0);
     }
     if (i[n] >= end) continue;

@@ -234,21 +234,40 @@ __device__ __forceinline__ float4 unpack4(uint32_t w, float s, bool root) {
 }
 
 // ------------------------------------------------------------------ scaling ---
-// Largest magnitude of the 8 values of each of a block's 16 lanes; NaN if one
-// is NaN. Every lane of the warp calls it.
-__device__ __forceinline__ float block_max(const V8& v) {
+// A lane holds N vectors of 8 elements of one block, so a block is 16 / N lanes
+// and a warp step 256 N elements. Vector k of a lane starts at this offset.
+template <int N>
+__device__ __forceinline__ int lane_offset(int lane, int k) {
+  constexpr int kLanes = 16 / N;
+  return (lane / kLanes) * kQ8Block + (lane % kLanes) * 8 + k * (8 * kLanes);
+}
+
+// Largest magnitude of a block; NaN if one is NaN. Every lane of the warp calls it.
+template <int N>
+__device__ __forceinline__ float block_max(const V8* v) {
   float m = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 x = f2_split(v.p[j]);
-    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(x.x), "f"(x.y));
+  for (int k = 0; k < N; ++k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = f2_split(v[k].p[j]);
+      asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(x.x), "f"(x.y));
+    }
   }
-  // one reduction of the whole warp for each half: half masks would run one after the other
-  const bool upper = (threadIdx.x & 16) != 0;
-  float lo, hi;
-  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(upper ? 0.0f : m));
-  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(upper ? m : 0.0f));
-  return upper ? hi : lo;
+  if (N == 1) {
+    // one reduction of the whole warp for each half: half masks would run one after the other
+    const bool upper = (threadIdx.x & 16) != 0;
+    float lo, hi;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(upper ? 0.0f : m));
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(upper ? m : 0.0f));
+    return upper ? hi : lo;
+  }
+#pragma unroll
+  for (int o = 8 / N; o > 0; o >>= 1) {
+    const float x = __shfl_xor_sync(0xffffffffu, m, o);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(x));
+  }
+  return m;
 }
 
 struct BlockScale {
@@ -320,7 +339,7 @@ __device__ __forceinline__ uint2 size_codes(const V8& x, const V8& rough, BlockS
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float2 y = f2_split(mul2(rough.p[j], f2(b.inv)));
-    const float2 t = f2_split(fma2(f2(sqrt_approx_ftz(fabsf(y.x)), sqrt_approx_ftz(fabsf(y.y))), f2(levels), f2(kPoint)));
+    const float2 t = f2_split(fma2(f2(sqrt_approx_ftz(ROOT ? y.x : fabsf(y.x)), sqrt_approx_ftz(ROOT ? y.y : fabsf(y.y))), f2(levels), f2(kPoint)));
     if (ROOT) asm("min.f32 %0, %0, %1, %2;" : "+f"(small) : "f"(t.x), "f"(t.y));
 #pragma unroll
     for (int e = 0; e < 2; ++e) {

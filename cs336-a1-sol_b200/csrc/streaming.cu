@@ -663,17 +663,24 @@ struct Front8Table {
   const float* gscale;
 };
 
-// What a warp step reads: loaded during the step before.
-template <typename T>
+// What a warp step (256 N elements, N vectors of 8 a lane) reads: loaded during
+// the step before.
+template <typename T, int N>
 struct Front8In {
-  Raw8<T> g;
-  uint2 codes;
+  Raw8<T> g[N];
+  uint2 codes[N];
   float s;
-  __device__ __forceinline__ void load(const T* G, const void* B, const float* SC, int64_t i, int64_t end, bool vec,
-                                       bool in) {
-    g.load(G, i, end, vec);
-    codes = load_codes(B, i, end, vec);
-    s = in ? SC[i / kQ8Block] : 0.0f;
+  __device__ __forceinline__ void load(const T* G, const void* B, const float* SC, int64_t tile, int lane, int64_t end,
+                                       bool aligned, bool full) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t i = tile + lane_offset<N>(lane, k);
+      const bool vec = full || (aligned && i + 8 <= end);
+      g[k].load(G, i, end, vec);
+      codes[k] = load_codes(B, i, end, vec);
+    }
+    const int64_t i = tile + lane_offset<N>(lane, 0);
+    s = full || i < end ? SC[i / kQ8Block] : 0.0f;
   }
 };
 struct Front8Args {
@@ -682,57 +689,68 @@ struct Front8Args {
   uint32_t step;
 };
 
-// One warp step: 256 elements, 8 a lane. FULL: all exist, vector accesses.
-template <typename T, bool REPAIR, bool NESTEROV, bool CLIP, bool FULL>
-__device__ __forceinline__ void front8_tile(const Front8In<T>& in8, const Front8Args& a, void* B, float* SC, uint16_t* U,
-                                            int64_t i, int64_t end, bool aligned, F2& acc) {
-  const bool vec = FULL || (aligned && i + 8 <= end);
-  const bool in = FULL || i < end;
-  Raw8<T> graw = in8.g;
-  V8 g = graw.get();
-  if (CLIP) {
+// FULL: all of a step's elements exist, vector accesses.
+template <typename T, bool REPAIR, bool NESTEROV, bool CLIP, bool FULL, int N>
+__device__ __forceinline__ void front8_tile(const Front8In<T, N>& in8, const Front8Args& a, void* B, float* SC,
+                                            uint16_t* U, int64_t tile, int lane, int64_t end, bool aligned, F2& acc) {
+  V8 g[N], m[N];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g.p[j] = mul2(g.p[j], f2(a.gs));
-    graw.set(g);
-    g = graw.get();
+  for (int k = 0; k < N; ++k) {
+    Raw8<T> graw = in8.g[k];
+    g[k] = graw.get();
+    if (CLIP) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[k].p[j] = mul2(g[k].p[j], f2(a.gs));
+      graw.set(g[k]);
+      g[k] = graw.get();
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[k].p[j] = mul2(f2(a.w1), g[k].p[j]);
+    m[k] = unpack_signed(in8.codes[k], in8.s);
+    if (!REPAIR) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m[k].p[j] = mul_add2(f2(a.beta), m[k].p[j], g[k].p[j], a.one);
+    }
   }
+  BlockScale b;
+  if (!REPAIR) b = signed_scale(block_max<N>(m));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) g.p[j] = mul2(f2(a.w1), g.p[j]);
-  V8 m = unpack_signed(in8.codes, in8.s);
-  if (!REPAIR) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m.p[j] = mul_add2(f2(a.beta), m.p[j], g.p[j], a.one);
-    const BlockScale b = signed_scale(block_max(m));
-    const uint2 codes = pack_signed<true>(m, b, dither_of(i, a.step));
-    if (in) {
+  for (int k = 0; k < N; ++k) {
+    const int64_t i = tile + lane_offset<N>(lane, k);
+    if (!FULL && i >= end) continue;  // (the warp's last step)
+    const bool vec = FULL || (aligned && i + 8 <= end);
+    if (!REPAIR) {
+      const uint2 codes = pack_signed<true>(m[k], b, dither_of(i, a.step));
       store_codes(B, i, end, vec, codes);
-      if ((threadIdx.x & 15) == 0) SC[i / kQ8Block] = b.s;
+      m[k] = unpack_signed(codes, b.s);
     }
-    m = unpack_signed(codes, b.s);
-  }
-  if (NESTEROV) {
+    if (NESTEROV) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m.p[j] = mul_add2(f2(a.beta), m.p[j], g.p[j], a.one);
-  }
-  Raw8<uint16_t> u;
-  u.set(m);
-  if (!in) return;  // (the warp's last step)
-  m = u.get();      // u as bf16 values
-#pragma unroll
-  for (int j = 0; j < 4; ++j) acc = fma2(m.p[j], m.p[j], acc);  // elements behind the end are 0
-  if (a.x0) {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 x = f2_split(mul2(m.p[j], f2(a.kx)));
-      w[j] = f32_to_f16(x.x) | static_cast<uint32_t>(f32_to_f16(x.y)) << 16;
+      for (int j = 0; j < 4; ++j) m[k].p[j] = mul_add2(f2(a.beta), m[k].p[j], g[k].p[j], a.one);
     }
-    u.a = make_uint4(w[0], w[1], w[2], w[3]);
+    Raw8<uint16_t> u;
+    u.set(m[k]);
+    const V8 x = u.get();  // u as bf16 values
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = fma2(x.p[j], x.p[j], acc);  // elements behind the end are 0
+    if (a.x0) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 y = f2_split(mul2(x.p[j], f2(a.kx)));
+        w[j] = f32_to_f16(y.x) | static_cast<uint32_t>(f32_to_f16(y.y)) << 16;
+      }
+      u.a = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    u.store(U, i, end, vec);
   }
-  u.store(U, i, end, vec);
+  if (!REPAIR && lane % (16 / N) == 0) {
+    const int64_t i = tile + lane_offset<N>(lane, 0);
+    if (FULL || i < end) SC[i / kQ8Block] = b.s;
+  }
 }
 
-template <typename T, bool REPAIR, bool NESTEROV, bool CLIP>
+template <typename T, bool REPAIR, bool NESTEROV, bool CLIP, int N>
 __device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, float beta, float w1, float one) {
   const MultiBatchInfo& bi = tab.h.b[find_batch_cta(tab.h, cta)];
   const int local = cta - bi.cta0;
@@ -752,25 +770,25 @@ __device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, flo
   // clipped gradient g = dtype(g * coef), as torch._foreach_mul_ leaves it
   a.gs = CLIP ? *tab.gscale : 1.0f;
   a.step = tab.step[bi.mat0 + s];
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   F2 acc = f2(0.0f);
-  const int64_t i0 = base + (threadIdx.x >> 5) * kQ8Tile + lane * 8;
-  constexpr int kStride = (kFrontThreads / 32) * kQ8Tile;
   if (bi.vec_ok && base + kFrontPart <= rc) {
-    Front8In<T> next;
-    next.load(G, B, SC, i0, end, true, true);
-#pragma unroll 2
-    for (int n = 0; n < kFrontPart / kStride; ++n) {
-      const Front8In<T> mine = next;
-      if (n + 1 < kFrontPart / kStride) next.load(G, B, SC, i0 + (n + 1) * kStride, end, true, true);
-      front8_tile<T, REPAIR, NESTEROV, CLIP, true>(mine, a, B, SC, U, i0 + n * kStride, end, true, acc);
+    constexpr int kStride = (kFrontThreads / 32) * (N * kQ8Tile);
+    int64_t tile = base + warp * (N * kQ8Tile);
+    Front8In<T, N> next;
+    next.load(G, B, SC, tile, lane, end, true, true);
+#pragma unroll 1
+    for (int n = 0; n < kFrontPart / kStride; ++n, tile += kStride) {
+      const Front8In<T, N> mine = next;
+      if (n + 1 < kFrontPart / kStride) next.load(G, B, SC, tile + kStride, lane, end, true, true);
+      front8_tile<T, REPAIR, NESTEROV, CLIP, true, N>(mine, a, B, SC, U, tile, lane, end, true, acc);
     }
   } else {
 #pragma unroll 1
-    for (int64_t i = i0; i - lane * 8 < end; i += kStride) {
-      Front8In<T> mine;
-      mine.load(G, B, SC, i, end, bi.vec_ok && i + 8 <= end, i < end);
-      front8_tile<T, REPAIR, NESTEROV, CLIP, false>(mine, a, B, SC, U, i, end, bi.vec_ok != 0, acc);
+    for (int64_t tile = base + warp * kQ8Tile; tile < end; tile += (kFrontThreads / 32) * kQ8Tile) {
+      Front8In<T, 1> mine;
+      mine.load(G, B, SC, tile, lane, end, bi.vec_ok != 0, false);
+      front8_tile<T, REPAIR, NESTEROV, CLIP, false, 1>(mine, a, B, SC, U, tile, lane, end, bi.vec_ok != 0, acc);
     }
   }
   if (REPAIR) return;
@@ -780,7 +798,7 @@ __device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, flo
   __shared__ float red[kFrontThreads / 32];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) pacc += __shfl_xor_sync(0xffffffffu, pacc, o);
-  if (lane == 0) red[threadIdx.x >> 5] = pacc;
+  if (lane == 0) red[warp] = pacc;
   __syncthreads();
   if (threadIdx.x == 0) {
     float t = 0.f;
@@ -789,11 +807,17 @@ __device__ __forceinline__ void front8_body(const Front8Table& tab, int cta, flo
   }
 }
 
+// 16 elements a lane and 3 CTAs an SM: the scale of a block, addresses and the
+// loop are paid for half as often as with 8 (33 instructions an element against
+// 38; 33.5 M elements, bf16 gradients: 42.8 us against 47.8; fp32: 45.8 against
+// 48.6). It is issue-bound (76 % of the slots) at 73 % of copy bandwidth for
+// bf16 and near the memory bound (90 %) for fp32.
+constexpr int kFront8Vecs = 2;
 template <typename T, bool NESTEROV, bool CLIP>
-__global__ void __launch_bounds__(kFrontThreads, CLIP ? 4 : 5) normuon_front8_kernel(const __grid_constant__ Front8Table tab,
+__global__ void __launch_bounds__(kFrontThreads, 3) normuon_front8_kernel(const __grid_constant__ Front8Table tab,
                                                                           float beta, float w1, float one) {
   pdl_wait();
-  front8_body<T, false, NESTEROV, CLIP>(tab, blockIdx.x, beta, w1, one);
+  front8_body<T, false, NESTEROV, CLIP, kFront8Vecs>(tab, blockIdx.x, beta, w1, one);
 }
 
 template <typename T, bool NESTEROV, bool CLIP>
@@ -808,7 +832,7 @@ __global__ void __launch_bounds__(kFrontThreads) normuon_x0_repair8_kernel(const
   const int s = m - bi.mat0;
   if (!bi.x0_half || !bi.flags[s]) return;
   for (int part = sub; part < bi.nparts; part += kRepairCtas)
-    front8_body<T, true, NESTEROV, CLIP>(tab, bi.cta0 + s * bi.nparts + part, beta, w1, one);
+    front8_body<T, true, NESTEROV, CLIP, 1>(tab, bi.cta0 + s * bi.nparts + part, beta, w1, one);
 }
 
 template <typename T>
