@@ -227,6 +227,9 @@ class AdamW(torch.optim.Optimizer):
             if step_of.setdefault(gi, self._steps.get(id(p), 0)) != self._steps.get(id(p), 0):
                 raise RuntimeError("params of one group have different step counts")
             buckets.setdefault((p.device, p.dtype, st["exp_avg"].dtype), []).append((gi, p, st))
+        for (_, _, sdt), members in buckets.items():
+            if sdt == torch.int8 and len({id(p) for _, p, _ in members}) != len(members):
+                raise ValueError("AdamW: a parameter with 8-bit moments appears twice")
         launches, ema_idx = [], set()
         pos = {id(p): i for i, p in enumerate(ps)}
         # (gradient words of a descriptor array, the items' positions in ps, byte offsets)

@@ -510,7 +510,8 @@ class NorMuonGNS(torch.optim.Optimizer):
         nesterov = int(bool(group["nesterov"]))
         gs = self._grad_scale.data_ptr() if self._grad_scale is not None else None
         for arr, n, dtc, dev, x0, m8 in plan["front"]:
-            self._front_call(lib, arr, n, dtc, beta, nesterov, gs, dev, x0, m8)
+            with _lib.on_device(dev):
+                self._front_call(lib, arr, n, dtc, beta, nesterov, gs, dev, x0, m8)
         ns_steps = int(group["ns_steps"])
         coeffs, resets, nres = self._table(ns_steps)
         mode = 0 if self.orthogonalizer == "quintic" else 1
@@ -520,8 +521,9 @@ class NorMuonGNS(torch.optim.Optimizer):
                 e0 = torch.cuda.Event(enable_timing=True)
                 e0.record()
                 n0 = _lib.launch_count()
-            rc = lib.b2o_orthogonalize_multi(groups, n, mode, coeffs, ns_steps, resets, nres, self.norm_eps,
-                                             self.norm_safety, wsb.data_ptr(), wsb.numel(), _lib.stream_ptr(dev))
+            with _lib.on_device(dev):
+                rc = lib.b2o_orthogonalize_multi(groups, n, mode, coeffs, ns_steps, resets, nres, self.norm_eps,
+                                                 self.norm_safety, wsb.data_ptr(), wsb.numel(), _lib.stream_ptr(dev))
             _lib.check(rc, "orthogonalize_multi")
             if ev is not None:
                 e1 = torch.cuda.Event(enable_timing=True)
@@ -530,9 +532,10 @@ class NorMuonGNS(torch.optim.Optimizer):
         beta2 = float(group["beta2"])
         lr, wd = float(group["lr"]), float(group["weight_decay"])
         for arr, n, dtc, dev in plan["apply"]:
-            rc = lib.b2o_normuon_apply_multi(arr, n, dtc, -lr, lr * wd, 1.0 - lr * wd, 1 if wd else 0,
-                                             int(bool(self.cautious_wd and wd)), 1.0 - beta2, self._ema_weight,
-                                             _lib.stream_ptr(dev))
+            with _lib.on_device(dev):
+                rc = lib.b2o_normuon_apply_multi(arr, n, dtc, -lr, lr * wd, 1.0 - lr * wd, 1 if wd else 0,
+                                                 int(bool(self.cautious_wd and wd)), 1.0 - beta2, self._ema_weight,
+                                                 _lib.stream_ptr(dev))
             _lib.check(rc, "normuon_apply")
         if self._ema is not None and plan["ema_idx"]:
             self._ema._folded |= plan["ema_idx"]
@@ -556,6 +559,8 @@ class NorMuonGNS(torch.optim.Optimizer):
                 params.append(p)
             if not params:
                 continue
+            if self.momentum_dtype is not None and len({id(p) for p in params}) != len(params):
+                raise ValueError("NorMuonGNS: a parameter with an 8-bit momentum appears twice")
             if hooked:
                 by_shape = OrderedDict()  # exact-shape buckets in param order (sol_modules.py:380-383)
                 for p in params:

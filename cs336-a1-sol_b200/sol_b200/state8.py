@@ -125,6 +125,8 @@ def decode(items, dtype=torch.float32, out=None):
     many = isinstance(dtype, (list, tuple))
     if many and len(dtype) != len(items):
         raise ValueError(f"state8.decode: {len(items)} states and {len(dtype)} dtypes")
+    if out is not None and len({t.data_ptr() for t in out if t.numel()}) != sum(1 for t in out if t.numel()):
+        raise ValueError("state8.decode: an output appears twice")
     values, rows = [], Rows()
     for i, (codes, scales, kind) in enumerate(items):
         code = _kind(kind)

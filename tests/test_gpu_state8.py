@@ -184,6 +184,8 @@ def test_conversions_refuse_what_does_not_fit(cuda):
         state8.decode([(q, s, "signed")], dtype=torch.float64)
     with pytest.raises(ValueError, match="size"):
         state8.decode([(q, s, "signed")], out=[x[:299]])
+    with pytest.raises(ValueError, match="twice"):
+        state8.decode([(q, s, "signed"), (q, s, "signed")], out=[x, x])
 
 
 # -------------------------------------------------------------------- AdamW --
@@ -354,6 +356,67 @@ def test_a_gradient_that_is_not_finite_stays_in_its_block(cuda):
         assert p.detach()[ok].isfinite().all()
         m, = [x["exp_avg_sq"] for x in opt.expanded_state()]
         assert m[256:384].isnan().all() and m[ok].isfinite().all()
+
+
+@pytest.mark.parametrize("size", [1e-20, 3e-19, 1e-12, 1e10])
+def test_moments_at_the_ends_of_the_range(cuda, size):
+    """Gradients whose squares are subnormal, and an eps of 0 that does not cover them; and large ones."""
+    g = _gen(6)
+    x = torch.randn(2000, generator=g) * size
+    x[torch.rand(2000, generator=g) < 0.1] *= 1e-3
+    p = torch.nn.Parameter(torch.zeros(2000, device=cuda))
+    opt = _optimizer([p], eps=0.0, lr=0.25)
+    st = {"exp_avg": torch.zeros(2000, dtype=torch.int8), "exp_avg_sq": torch.zeros(2000, dtype=torch.uint8),
+          "exp_avg_scale": torch.zeros(16), "exp_avg_sq_scale": torch.zeros(16)}
+    for step in range(1, 4):
+        before = p.detach().cpu()
+        p.grad = x.cuda()
+        opt.step()
+        w = ref.adamw_step(before, None, x, st, lr=0.25, betas=(0.9, 0.95), eps=0.0, wd=0.0, cautious=False, step=step)
+        for k in KEYS:
+            assert torch.equal(opt.state[p][k].cpu(), st[k]), (k, step)
+        got, up = p.detach().cpu().double(), (w - before.double()).abs()
+        ok = w.isfinite()  # a square that has become 0 leaves m / 0, as in 32 bits
+        assert ((got - w).abs() <= 64 * 2.0 ** -24 * up + 4 * 2.0 ** -24 * (before.double().abs() + w.abs()))[ok].all()
+        assert ok.any()
+        if not ok.all():
+            break
+
+
+def test_a_parameter_twice_is_refused(cuda):
+    p = torch.nn.Parameter(torch.zeros(64, 128, device=cuda))
+    p.grad = torch.ones_like(p)
+    with pytest.warns(UserWarning, match="duplicate"):
+        opt = _optimizer([p, p])
+    with pytest.raises(ValueError, match="twice"):
+        opt.step()
+    with pytest.warns(UserWarning, match="duplicate"):
+        muon = NorMuonGNS([p, p], momentum_dtype=torch.int8)
+    with pytest.raises(ValueError, match="twice"):
+        muon.step()
+
+
+def test_two_optimizers_take_turns(cuda):
+    """Steps of two optimizers in turn, with a conversion between them, equal each run alone."""
+    def make(seed):
+        ps = [torch.nn.Parameter(x.cuda()) for x in _tensors(torch.bfloat16, seed, [(64, 300), (4099,)])]
+        return ps, _optimizer(ps, master="bf16_mt")
+    alone = []
+    for seed in (1, 2):
+        ps, opt = make(seed)
+        for step in range(3):
+            for p, x in zip(ps, _grads(ps, 10 * seed + step)):
+                p.grad = x.cuda()
+            opt.step()
+        alone.append([p.detach() for p in ps])
+    pair = [make(1), make(2)]
+    for step in range(3):
+        for seed, (ps, opt) in zip((1, 2), pair):
+            for p, x in zip(ps, _grads(ps, 10 * seed + step)):
+                p.grad = x.cuda()
+            opt.step()
+            opt.expanded_state(dtype=torch.bfloat16)
+    assert all(torch.equal(a, p) for ps, b in zip([x[0] for x in pair], alone) for a, p in zip(b, ps))
 
 
 def test_small_tensors_keep_wide_moments(cuda):
