@@ -272,23 +272,26 @@ __device__ __forceinline__ float block_max(const V8* v) {
 
 struct BlockScale {
   float s;      // the scale that is stored
-  float inv;    // 1 / s, or 4 / s from s = 1 on (1 / s would become subnormal); 0 where every code is 0
+  float inv;    // 1 / s (signed, from s = 1 on: 4 / s, since 1 / s may be subnormal); 0 where every code is 0
   float half;   // 1, or 1/2 to go with 4 / s: sqrt(x / s) = half sqrt(x inv)
+  float tie;    // the state whose size is s / 4, midway between the two middle codes
 };
-__device__ __forceinline__ BlockScale finish_scale(float s) {
+__device__ __forceinline__ BlockScale signed_scale(float top) {
   BlockScale b;
-  const bool big = s >= 1.0f;
-  b.s = s;
-  b.inv = s > 0.0f ? rcp_approx_ftz(big ? 0.25f * s : s) : 0.0f;
+  b.s = !(top < __int_as_float(0x7f800000)) ? __int_as_float(0x7fffffff) : top < 1.17549435e-38f ? 0.0f : top;
+  const bool big = b.s >= 1.0f;
+  b.inv = b.s > 0.0f ? rcp_approx_ftz(big ? 0.25f * b.s : b.s) : 0.0f;
   b.half = big ? 0.5f : 1.0f;
+  b.tie = 0.25f * b.s;
   return b;
 }
-__device__ __forceinline__ BlockScale signed_scale(float top) {
-  return finish_scale(!(top < __int_as_float(0x7f800000)) ? __int_as_float(0x7fffffff)
-                                                          : top < 1.17549435e-38f ? 0.0f : top);
-}
-__device__ __forceinline__ BlockScale root_scale(float top) {
-  return finish_scale(!(top < __int_as_float(0x7f800000)) ? __int_as_float(0x7fffffff) : __fsqrt_rn(top));
+__device__ __forceinline__ BlockScale root_scale(float top) {  // roots lie between 2^-75 and 2^64
+  BlockScale b;
+  b.s = !(top < __int_as_float(0x7f800000)) ? __int_as_float(0x7fffffff) : __fsqrt_rn(top);
+  b.inv = b.s > 0.0f ? rcp_approx_ftz(b.s) : 0.0f;
+  b.half = 1.0f;
+  b.tie = 0.0625f * top;
+  return b;
 }
 
 // ------------------------------------------------------------------ writing ---
@@ -359,7 +362,12 @@ __device__ __forceinline__ uint2 size_codes(const V8& x, const V8& rough, BlockS
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t at = q[k] & 0xffffffu;
-      if ((at & 0xffffu) < 2 * kSlack || (ROOT && at < 0x20000u)) todo |= 1u << k;
+      const float2 pair = f2_split(x.p[k / 2]);
+      // u = 1/2: a size of exactly s / 4 lies on the border and has the integer
+      // part already (levels / 2 + 1/2, rounded up). Among bf16 states one in
+      // 700 is such a tie.
+      const bool tie = !DITHER && fabsf(k & 1 ? pair.y : pair.x) == b.tie;
+      if (((at & 0xffffu) < 2 * kSlack && !tie) || (ROOT && at < 0x20000u)) todo |= 1u << k;
     }
     while (todo) {
       const int k = __ffs(todo) - 1;
