@@ -35,8 +35,8 @@ struct Adam8Coef {
   uint32_t turn;                  // the step count that the codes' offsets run with
   float one;                      // 1 (see mul_add2)
   int wd_on, cautious;
-  // 1: roots of subnormal second moments may read as 0 in the update (eps
-  // covers them by 2^24 times); 0: they are computed (a few instructions more)
+  // 1: the roots of subnormal second moments may read as 0 in the update (eps
+  // covers them 2^24 times); 0: they are computed, and the division is IEEE's
   int plain_roots;
   const float* grad_scale;
 };
@@ -61,9 +61,9 @@ __device__ __forceinline__ int find_tensor(const Table& tab, int chunk) {
 }
 
 // One warp step: 256 elements, 8 a lane, blocks of 16 lanes.
-// FULL: all of them exist and every pointer takes vector accesses; EXTRA: the
-// group may have a clip coefficient, weight decay or an eps that does not cover
-// subnormal roots.
+// FULL: all of them exist and every pointer takes vector accesses. EXTRA 1: a
+// group may have a clip coefficient or weight decay; 2: also an eps that does not
+// cover the roots of subnormal second moments (see plain_roots).
 // `mine` are the step's first inputs, loaded during the step before.
 template <typename PT>
 struct Adam8In {
@@ -79,7 +79,7 @@ struct Adam8In {
   }
 };
 
-template <typename PT, bool REM, bool EMA, bool EXTRA, bool FULL>
+template <typename PT, bool REM, bool EMA, int EXTRA, bool FULL>
 __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Adam8Coef& c, float ema_weight,
                                             const Adam8In<PT>& mine, int64_t i, int64_t end, bool aligned, float gs) {
   const bool vec = FULL || (aligned && i + 8 <= end);
@@ -113,7 +113,7 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float2 x = f2_split(v.p[j]);
-    if (!EXTRA || c.plain_roots) r.p[j] = f2(sqrt_approx_ftz(x.x), sqrt_approx_ftz(x.y));
+    if (EXTRA < 2) r.p[j] = f2(sqrt_approx_ftz(x.x), sqrt_approx_ftz(x.y));
     else r.p[j] = f2(sqrt_approx(x.x), sqrt_approx(x.y));
   }
   if (!in) return;
@@ -126,16 +126,43 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
   if (EXTRA && c.wd_on) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 x = f2_split(w.p[j]), y = f2_split(m.p[j]);
-      const float kx = !c.cautious || x.x * y.x > 0.0f ? -c.lr_wd : 0.0f;
-      const float ky = !c.cautious || x.y * y.y > 0.0f ? -c.lr_wd : 0.0f;
-      w.p[j] = fma2(w.p[j], f2(kx, ky), w.p[j]);
+      if (c.cautious) {
+        const float2 x = f2_split(w.p[j]), y = f2_split(m.p[j]);
+        w.p[j] = mul2(w.p[j], f2(x.x * y.x > 0.0f ? 1.0f - c.lr_wd : 1.0f, x.y * y.y > 0.0f ? 1.0f - c.lr_wd : 1.0f));
+      } else {
+        w.p[j] = mul_add2(w.p[j], f2(-c.lr_wd), w.p[j], c.one);
+      }
     }
   }
+  // w -= step_size m / (sqrt(v) inv_bc2 + eps), each operation rounded by itself.
+  // The quotient is corrected by its residual (Markstein's step: q + (a - d q) /
+  // d), so it is the rounded one: where a second moment is 0 the denominator is
+  // eps alone, and an update that much larger than the weight would show the
+  // approximation in the stored bf16 bits. With a remainder the stored weight has
+  // twice the bits, and the root gets its residual step too (Newton: s + (v -
+  // s^2) / (2 s)); 0 and subnormal v keep the root 0.
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 d = f2_split(fma2(r.p[j], f2(c.inv_bc2), f2(c.eps)));
-    w.p[j] = fma2(mul2(m.p[j], f2(-c.step_size)), f2(rcp_approx_ftz(d.x), rcp_approx_ftz(d.y)), w.p[j]);
+    F2 root = r.p[j];
+    if (REM && EXTRA < 2) {
+      const float2 x = f2_split(v.p[j]);
+      const F2 inv = f2(fminf(rsqrt_approx_ftz(x.x), 9.2233720e18f), fminf(rsqrt_approx_ftz(x.y), 9.2233720e18f));
+      const F2 rest = fma2(mul2(root, f2(-1.0f)), root, v.p[j]);
+      root = fma2(rest, mul2(inv, f2(0.5f)), root);
+    }
+    const F2 minus_d = mul_add2(root, f2(-c.inv_bc2), f2(-c.eps), c.one);
+    const F2 a = mul2(m.p[j], f2(-c.step_size));
+    const float2 d = f2_split(minus_d);
+    F2 q;
+    if (EXTRA < 2) {
+      const F2 inv = f2(rcp_approx_ftz(-d.x), rcp_approx_ftz(-d.y));
+      q = mul2(a, inv);
+      q = fma2(fma2(minus_d, q, a), inv, q);
+    } else {  // (eps may be 0, and with it the denominator)
+      const float2 x = f2_split(a);
+      q = f2(__fdiv_rn(x.x, -d.x), __fdiv_rn(x.y, -d.y));
+    }
+    w.p[j] = add2(w.p[j], q);
   }
   praw.set(w);
   praw.store(P, i, end, vec);
@@ -166,8 +193,17 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
   }
 }
 
-template <typename PT, bool REM, bool EMA, bool EXTRA>
-__global__ void __launch_bounds__(kS8Threads, EMA ? 3 : 4) adamw8_kernel(const __grid_constant__ Adam8Table tab) {
+// 256 threads, a chunk of 8192 elements a CTA, 3 or 4 CTAs an SM (80 or 64
+// registers). Measured on 33.5 M elements (a 32768 x 1024 table), against copy
+// bandwidth: bf16 weights 69 us (75 %, bound by instruction issue: 57 an
+// element), with a remainder 85 us (85 %), with the EMA too 121 us (94 %); fp32
+// 84 us (98 %), with the EMA 123 us (100 %). The residual steps of quotient and
+// root cost 2 and 4 us where issue binds. Without the loads a step ahead the
+// first of these took 102 us; with 2 CTAs an SM 145; 16 elements a lane instead
+// of 8 took 19 % fewer instructions and the same time (fewer warps).
+template <typename PT, bool REM, bool EMA, int EXTRA>
+__global__ void __launch_bounds__(kS8Threads, EMA || EXTRA == 2 ? 3 : 4)
+    adamw8_kernel(const __grid_constant__ Adam8Table tab) {
   pdl_wait();
   const int ti = find_tensor(tab, blockIdx.x);
   const b2o_adamw8_tensor& T = tab.t[ti];
@@ -200,14 +236,17 @@ __global__ void __launch_bounds__(kS8Threads, EMA ? 3 : 4) adamw8_kernel(const _
   }
 }
 
+template <typename PT, bool REM, bool EMA>
+static void adamw8_launch(const Adam8Table& tab, int chunks, int extra, cudaStream_t stream) {
+  launch_pdl(extra == 2   ? adamw8_kernel<PT, REM, EMA, 2>
+             : extra == 1 ? adamw8_kernel<PT, REM, EMA, 1>
+                          : adamw8_kernel<PT, REM, EMA, 0>,
+             dim3(chunks), dim3(kS8Threads), 0, stream, tab);
+}
 template <typename PT, bool REM>
-static void adamw8_launch(const Adam8Table& tab, int chunks, bool ema, bool extra, cudaStream_t stream) {
-  if (ema)
-    launch_pdl(extra ? adamw8_kernel<PT, REM, true, true> : adamw8_kernel<PT, REM, true, false>, dim3(chunks),
-               dim3(kS8Threads), 0, stream, tab);
-  else
-    launch_pdl(extra ? adamw8_kernel<PT, REM, false, true> : adamw8_kernel<PT, REM, false, false>, dim3(chunks),
-               dim3(kS8Threads), 0, stream, tab);
+static void adamw8_launch(const Adam8Table& tab, int chunks, bool ema, int extra, cudaStream_t stream) {
+  if (ema) adamw8_launch<PT, REM, true>(tab, chunks, extra, stream);
+  else adamw8_launch<PT, REM, false>(tab, chunks, extra, stream);
 }
 
 int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8_group* groups, int ngroups,
@@ -228,7 +267,7 @@ int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8
     c.b1 = static_cast<float>(g.beta1); c.w1 = static_cast<float>(1.0 - g.beta1);
     c.b2 = static_cast<float>(g.beta2); c.w2 = static_cast<float>(1.0 - g.beta2);
     c.step_size = static_cast<float>(g.lr / (1.0 - std::pow(g.beta1, g.step)));
-    c.inv_bc2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(g.beta2, g.step)));
+    c.inv_bc2 = 1.0f / static_cast<float>(std::sqrt(1.0 - std::pow(g.beta2, g.step)));
     c.eps = static_cast<float>(g.eps);
     c.lr_wd = static_cast<float>(g.lr * g.weight_decay);
     c.step = static_cast<float>(g.step);
@@ -257,7 +296,7 @@ int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8
     const bool rem = (mix & 1) != 0, ema = (mix & 2) != 0;
     for (int at = 0; at < ntensors;) {
       int n = 0, chunks = 0;
-      bool extra = false;
+      int extra = 0;
       for (; at < ntensors && n < kS8Tensors; ++at) {
         const b2o_adamw8_tensor& t = tensors[at];
         if (t.numel == 0 || (t.rem != nullptr) != rem || (t.ema != nullptr) != ema) continue;
@@ -268,7 +307,7 @@ int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8
         tab.vec_ok[n] = aligned16(t.param) && aligned16(t.grad) && aligned8(t.exp_avg) && aligned8(t.exp_avg_sq) &&
                         (!t.rem || aligned16(t.rem)) && (!t.ema || aligned16(t.ema));
         const Adam8Coef& c = tab.g[t.group];
-        extra = extra || c.grad_scale || c.wd_on || !c.plain_roots;
+        extra = std::max(extra, !c.plain_roots ? 2 : c.grad_scale || c.wd_on ? 1 : 0);
         chunks += ch;
         ++n;
       }

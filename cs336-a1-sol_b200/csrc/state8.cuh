@@ -62,6 +62,11 @@ __device__ __forceinline__ float sqrt_approx_ftz(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float rsqrt_approx_ftz(float x) {  // relative error 2^-22.9
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ float rcp_approx_ftz(float x) {  // relative error 2^-23
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
