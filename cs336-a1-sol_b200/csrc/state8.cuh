@@ -18,17 +18,19 @@
 // become zero would stay at 9 of 127 codes for good. In a step, u therefore
 // runs evenly over [0, 1): u = h / 2^32 to 23 bits, h = A i + B t (+ 2^31 for
 // signed) mod 2^32 for element i of the tensor and step t, A = 2^32 / golden
-// ratio, B = 2^32 (sqrt 2 - 1): turns that leave no wide gap. The rounding is then right on average over steps, with no random
-// state to keep. Simulated updates (128-element blocks, lognormal scales of
-// the elements with sigma 0.3, betas 0.9 / 0.95, .99, .999) are off by 3.2, 3.5
-// and 3.8 % rms against 2.9, 6.3 and 5.4 % to nearest. A conversion (encode)
-// uses u = 1/2, so that what was decoded encodes to the same codes.
+// ratio, B = 2^32 (sqrt 2 - 1): turns that leave no wide gap. The rounding is
+// then right on average over steps, with no random state to keep. Simulated
+// updates (128-element blocks, lognormal scales of the elements with sigma 0.3,
+// betas 0.9 / 0.95, .99, .999) are off by 3.2, 3.5 and 3.8 % rms against 2.9, 6.3
+// and 5.4 % to nearest. A conversion (encode) uses u = 1/2, so that what was
+// decoded encodes to the same codes.
 //
 // A code is exact: it depends on nothing but the fp32 state, its block's fp32
 // scale and u. The fast path computes y = levels sqrt(x / s) with approximate
 // instructions (error below 1e-4) as a fixed-point number with 16 bits behind
 // the point, so that adding the top 16 bits of h leaves the code in one byte.
-// Where y + u lands within 8 (signed: 4) / 65536 of an integer K, the side is decided by comparing x levels^2 with s (K - u)^2 in 64 bits.
+// Where y + u lands within 8 (signed: 4) / 65536 of an integer K, the side is
+// decided by comparing x levels^2 with s (K - u)^2 in 64 bits.
 //
 // What bounds the passes that write codes is instruction issue, not memory: a
 // first form with scalar arithmetic and u added in floating point took 208 us
@@ -36,7 +38,7 @@
 // bandwidth) at 103 instructions an element. Hence the fixed point, packed pairs
 // of floats (two roundings an instruction, each as the scalar one), the block
 // maximum in reduction instructions, one kernel for each set of options, and
-// the next step's loads ahead of this one's work: 70 us at 56 instructions.
+// the next step's loads ahead of this one's work: 69 us at 57 instructions.
 //
 // Special blocks: a value that is not finite makes the scale NaN and every
 // code 0 (the whole block reads as NaN); s = 0 (for signed also s < 2^-126,
@@ -263,8 +265,9 @@ __device__ __forceinline__ float block_max(const V8* v) {
     // one reduction of the whole warp for each half: half masks would run one after the other
     const bool upper = (threadIdx.x & 16) != 0;
     float lo, hi;
-    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(upper ? 0.0f : m));
-    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(upper ? m : 0.0f));
+    // (volatile: every lane has to execute them, so they stay ahead of any branch)
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(upper ? 0.0f : m));
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(upper ? m : 0.0f));
     return upper ? hi : lo;
   }
 #pragma unroll
@@ -279,7 +282,7 @@ struct BlockScale {
   float s;      // the scale that is stored
   float inv;    // 1 / s (signed, from s = 1 on: 4 / s, since 1 / s may be subnormal); 0 where every code is 0
   float half;   // 1, or 1/2 to go with 4 / s: sqrt(x / s) = half sqrt(x inv)
-  float tie;    // the state whose size is s / 4, midway between the two middle codes
+  float tie;    // the state whose size is exactly s / 4, midway between the two middle codes (-1: none that small)
 };
 __device__ __forceinline__ BlockScale signed_scale(float top) {
   BlockScale b;
@@ -287,7 +290,7 @@ __device__ __forceinline__ BlockScale signed_scale(float top) {
   const bool big = b.s >= 1.0f;
   b.inv = b.s > 0.0f ? rcp_approx_ftz(big ? 0.25f * b.s : b.s) : 0.0f;
   b.half = big ? 0.5f : 1.0f;
-  b.tie = 0.25f * b.s;
+  b.tie = b.s >= 1e-36f ? 0.25f * b.s : -1.0f;
   return b;
 }
 __device__ __forceinline__ BlockScale root_scale(float top) {  // roots lie between 2^-75 and 2^64
@@ -295,7 +298,7 @@ __device__ __forceinline__ BlockScale root_scale(float top) {  // roots lie betw
   b.s = !(top < __int_as_float(0x7f800000)) ? __int_as_float(0x7fffffff) : __fsqrt_rn(top);
   b.inv = b.s > 0.0f ? rcp_approx_ftz(b.s) : 0.0f;
   b.half = 1.0f;
-  b.tie = 0.0625f * top;
+  b.tie = top >= 1e-36f ? 0.0625f * top : -1.0f;
   return b;
 }
 
@@ -332,9 +335,9 @@ __device__ __forceinline__ float pick8(const V8& v, int k) {
 // y's fixed point comes from adding 2^7 (2^8 for 255 levels, whose last place
 // is 2^-15) and kSlack / 65536: a sum within kSlack / 65536 of an integer on
 // either side then has the high bits of its fraction clear. kSlack covers, in
-// units of 2^-16: 2^-24 levels x (3 of the size or 2 of its root, 2 of 1 / s, 1
-// of their product, all halved by the root, 2 of the root), half a place of
-// the sum, 1 of cutting u to 16 bits: 3.3 of 4 and 7 of 8.
+// units of 2^-16: levels x 2^-24 x ((2 of a rough root, none of a size, + 2 of
+// 1 / s + 1 of their product) / 2 + 2 of the root), half a place of the sum (1/2;
+// ROOT 1), and 1 of cutting u to 16 bits: 3.3 of 4 and 6.5 of 8.
 template <bool DITHER, bool ROOT>
 __device__ __forceinline__ uint2 size_codes(const V8& x, const V8& rough, BlockScale b, uint32_t h) {
   constexpr uint32_t kSlack = ROOT ? 8 : 4;
@@ -347,7 +350,8 @@ __device__ __forceinline__ uint2 size_codes(const V8& x, const V8& rough, BlockS
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float2 y = f2_split(mul2(rough.p[j], f2(b.inv)));
-    const float2 t = f2_split(fma2(f2(sqrt_approx_ftz(ROOT ? y.x : fabsf(y.x)), sqrt_approx_ftz(ROOT ? y.y : fabsf(y.y))), f2(levels), f2(kPoint)));
+    const F2 ys = f2(sqrt_approx_ftz(ROOT ? y.x : fabsf(y.x)), sqrt_approx_ftz(ROOT ? y.y : fabsf(y.y)));
+    const float2 t = f2_split(fma2(ys, f2(levels), f2(kPoint)));
     if (ROOT) asm("min.f32 %0, %0, %1, %2;" : "+f"(small) : "f"(t.x), "f"(t.y));
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -359,8 +363,9 @@ __device__ __forceinline__ uint2 size_codes(const V8& x, const V8& rough, BlockS
   }
   uint2 out = make_uint2(pack4(q), pack4(q + 4));
   // the smallest fraction, two to a register
-  const uint32_t least2 = __vminu2(__vimin3_u16x2(prmt(q[0], q[1], 0x5410), prmt(q[2], q[3], 0x5410), prmt(q[4], q[5], 0x5410)),
-                                   prmt(q[6], q[7], 0x5410));
+  const uint32_t least2 = __vminu2(
+      __vimin3_u16x2(prmt(q[0], q[1], 0x5410), prmt(q[2], q[3], 0x5410), prmt(q[4], q[5], 0x5410)),
+      prmt(q[6], q[7], 0x5410));
   const uint32_t least = min(least2 & 0xffffu, least2 >> 16);
   if ((least < 2 * kSlack || (ROOT && small < kOne)) && b.inv > 0.0f) {
     uint32_t todo = 0;
@@ -386,10 +391,8 @@ __device__ __forceinline__ uint2 size_codes(const V8& x, const V8& rough, BlockS
       if (ROOT && near < 2) {
         // A live state keeps a code. One this small may have lost its rough
         // size to 0, and the largest's sum may have wrapped past 2^24 to here.
-        if (v > 0.0f)
-          code = max(1, static_cast<int>(255.0 * sqrt(static_cast<double>(__fsqrt_rn(v)) / static_cast<double>(b.s)) + u));
-        else
-          code = 0;
+        const double y = 255.0 * sqrt(static_cast<double>(__fsqrt_rn(v)) / static_cast<double>(b.s));
+        code = v > 0.0f ? max(1, static_cast<int>(y + u)) : 0;
       } else {
         code = near_code(ROOT ? __fsqrt_rn(v) : fabsf(v), b.s, near, kLevels, u);
       }

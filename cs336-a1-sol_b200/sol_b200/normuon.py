@@ -276,6 +276,9 @@ class NorMuonGNS(torch.optim.Optimizer):
         keeps them alive."""
         if self.momentum_dtype is None:
             return None
+        for b in members:
+            for p, st in zip(b["params"], b["states"]):
+                state8.check_state(p, st["momentum_buffer"], st["momentum_scale"], "signed", "NorMuonGNS: momentum_buffer")
         scales = [_lib.ptr_array([st["momentum_scale"].data_ptr() for st in b["states"]]) for b in members]
         steps = [np.zeros(b["S"], dtype=np.uint32) for b in members]
         return (_lib.ptr_array([_lib.addr(x) for x in scales]), _lib.ptr_array([x.ctypes.data for x in steps]),

@@ -71,6 +71,13 @@ def _check_codes(codes, scales, kind, n, what):
                          f"{want[1]} {want[0]} scales (got {codes.dtype}, {scales.numel()} {scales.dtype})")
 
 
+def check_state(p, codes, scales, kind, what):
+    """Refuses a state that does not belong to parameter p (a loaded one may not)."""
+    if codes.numel() != p.numel() or codes.get_device() != p.get_device():
+        raise ValueError(f"{what}: {codes.numel()} codes for a parameter of {p.numel()} elements, or on another device")
+    _check_codes(codes, scales, kind, p.numel(), what)
+
+
 class Rows:
     """Descriptors of one call (b2o_state_tensor as 64-bit words), by device."""
     __slots__ = ("by",)
@@ -118,7 +125,8 @@ def decode(items, dtype=torch.float32, out=None):
     """[(codes, scales, kind), ...] -> values, in the shape of the codes.
 
     ``dtype``: torch.float32 or torch.bfloat16 (nearest), one for all or a list.
-    ``out``: contiguous tensors to write instead of new ones (their dtype counts)."""
+    ``out``: contiguous tensors to write instead of new ones (their dtype counts);
+    they may not overlap."""
     items = list(items)
     if out is not None and len(out) != len(items):
         raise ValueError(f"state8.decode: {len(items)} states and {len(out)} outputs")

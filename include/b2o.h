@@ -145,7 +145,8 @@ int b2o_state_decode(const b2o_state_tensor* tensors, int ntensors, void* stream
  * exp_avg_sq ROOT. The update uses the moments before they are rounded to 8
  * bits. A tensor may be a slice of a larger one that starts at a multiple of
  * B2O_STATE_BLOCK and ends at one or at the larger tensor's end (every pointer
- * at the slice's first element or block): the result is then that of the whole. */
+ * at the slice's first element or block): the result is then that of the whole.
+ * No element may be listed twice. */
 typedef struct {
   void* param;             /* param_dtype, numel elements                 */
   uint16_t* rem;           /* bf16 remainder of a bf16 weight, or NULL    */

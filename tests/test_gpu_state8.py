@@ -47,6 +47,8 @@ def _values(n, root, what, seed=0):
     elif what == "quarters":  # the middle between two codes, exactly
         x = torch.where(torch.rand(n, generator=g) < 0.5, 0.25, -0.25)
         x[::97] = 1.0
+    elif what == "least":  # ties and scales where a quarter is no longer exact
+        x = torch.where(torch.rand(n, generator=g) < 0.5, 2.0 ** -128, 2.0 ** -126 * (1 + 2.0 ** -23)) * (1 + (x > 0))
     elif what == "same":
         x.fill_(-0.37)
     elif what == "sparse":
@@ -62,7 +64,7 @@ def _same(a, b):
 # ------------------------------------------------------------ encode/decode --
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("root", [False, True])
-@pytest.mark.parametrize("what", ["normal", "zeros", "spike", "subnormal", "tiny", "huge", "quarters", "same", "sparse"])
+@pytest.mark.parametrize("what", ["normal", "zeros", "spike", "subnormal", "tiny", "huge", "quarters", "least", "same", "sparse"])
 def test_encode_and_decode_match_the_definition(cuda, what, root, dtype):
     kind = "root" if root else "signed"
     xs = [_values(n, root, what, seed=n).to(dtype) for n in SIZES]
@@ -82,7 +84,7 @@ def test_encode_and_decode_match_the_definition(cuda, what, root, dtype):
         y = (255 if root else 127) * ((x.double().sqrt() if root else x.double().abs()) / top.clamp(min=1e-300)).sqrt()
         yv = (255 if root else 127) * ((rv.double().sqrt() if root else rv.double().abs()) / top.clamp(min=1e-300)).sqrt()
         live = ok & (top > 0) & (rv != 0)
-        assert ((y - yv).abs()[live] <= torch.where(y < 0.5, 1.0, 0.5001)[live]).all() or what in ("subnormal", "tiny")
+        assert ((y - yv).abs()[live] <= torch.where(y < 0.5, 1.0, 0.5001)[live]).all() or what in ("subnormal", "tiny", "least")
 
 
 @pytest.mark.parametrize("root", [False, True])
@@ -435,6 +437,31 @@ def test_a_master_weight_is_the_rounded_update(cuda):
             w = full.to(torch.bfloat16)
             rem = (full - w.float()).to(torch.bfloat16)
             assert (p.detach().cpu() != w).sum() <= 2 and (opt.state[p]["mant_rem"].cpu() != rem).sum() <= 2, (wd, step)
+
+
+def test_a_state_of_another_size_is_refused(cuda):
+    """Codes or scales that do not belong to the parameter (a damaged checkpoint) never reach a kernel."""
+    p = torch.nn.Parameter(torch.zeros(64, 128, device=cuda))
+    p.grad = torch.ones_like(p)
+    opt, muon = _optimizer([p]), NorMuonGNS([p], momentum_dtype=torch.int8)
+    opt.step()
+    muon.step()
+    for o, keys in ((opt, ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")),
+                    (muon, ("momentum_buffer", "momentum_scale"))):
+        for k in keys:
+            good = o.state[p][k]
+            for bad in (good[:-1].clone(), good.to(torch.int16 if good.dtype != torch.float32 else torch.bfloat16)):
+                o.state[p][k] = bad
+                o.invalidate_plan()
+                with pytest.raises((ValueError, TypeError)):
+                    o.step()
+            o.state[p][k] = good
+        o.invalidate_plan()
+        o.step()
+    opt.state[p]["exp_avg"] = torch.zeros(64, 128, device=cuda)  # wide beside 8 bits
+    opt.invalidate_plan()
+    with pytest.raises(ValueError, match="one dtype"):
+        opt.step()
 
 
 def test_a_parameter_twice_is_refused(cuda):
