@@ -163,29 +163,34 @@ class AdamW(torch.optim.Optimizer):
         value_code = state8._VALUE_CODE.get(dtype)
         if value_code is None:
             raise TypeError(f"AdamW.expanded_state: float32 or bfloat16 (got {dtype})")
-        out, rows, eight, empty = [], state8.Rows(), torch.int8, torch.empty_like
+        signed, root = value_code << 32, 1 | value_code << 32
+        pair = 2 | _lib.F32 << 32
+        out, rows, last, extend = [], state8.Rows(), None, None
+        empty, eight, f32, states = torch.empty_like, torch.int8, torch.float32, self.state
         for p in params:
-            if not p.is_cuda:
+            index = p.get_device()
+            if index != last:
                 _lib.require_cuda(p, "AdamW.expanded_state")
-            st = self.state.get(p)
+                last, extend = index, rows.extend(index)
+            st = states.get(p)
             if not st or "exp_avg" not in st:
                 st = self._init_state(p)
             m, v, n = st["exp_avg"], st["exp_avg_sq"], p.numel()
-            wide = {}
-            if m.dtype == eight:
-                wide["exp_avg"], wide["exp_avg_sq"] = a, b = empty(m, dtype=dtype), empty(v, dtype=dtype)
+            if m.dtype is eight:
+                a, b = empty(m, dtype=dtype), empty(v, dtype=dtype)
                 if n:
-                    rows.add(a, m, st["exp_avg_scale"], n, 0, value_code)
-                    rows.add(b, v, st["exp_avg_sq_scale"], n, 1, value_code)
+                    extend((a.data_ptr(), m.data_ptr(), st["exp_avg_scale"].data_ptr(), n, signed,
+                            b.data_ptr(), v.data_ptr(), st["exp_avg_sq_scale"].data_ptr(), n, root))
             else:
-                wide["exp_avg"], wide["exp_avg_sq"] = m.to(dtype, copy=True), v.to(dtype, copy=True)
+                a, b = m.to(dtype, copy=True), v.to(dtype, copy=True)
+            wide = {"exp_avg": a, "exp_avg_sq": b}
             rem = st.get("mant_rem")
             if rem is not None:
                 if not p.is_contiguous():
                     raise ValueError("AdamW.expanded_state: contiguous parameters only")
-                wide["master"] = w = empty(rem, dtype=torch.float32)
+                wide["master"] = w = empty(rem, dtype=f32)
                 if n:
-                    rows.add(w, p, rem, n, 2, _lib.F32)
+                    extend((w.data_ptr(), p.data_ptr(), rem.data_ptr(), n, pair))
             out.append(wide)
         rows.launch(_lib.load().b2o_state_decode, "state_decode")
         return out

@@ -60,15 +60,18 @@ def _value_code(t, what) -> int:
 
 
 def _check_codes(codes, scales, kind, n, what):
-    if not (codes.is_cuda and scales.is_cuda):
-        _lib.require_cuda(codes, what)
-        _lib.require_cuda(scales, what)
+    pair = kind == "pair"
+    if (codes.dtype is _CODE_DTYPE[kind] and scales.dtype is (torch.bfloat16 if pair else torch.float32) and
+            scales.numel() == (n if pair else (n + BLOCK - 1) // BLOCK) and codes.is_cuda and
+            codes.get_device() == scales.get_device() and codes.is_contiguous() and scales.is_contiguous()):
+        return
+    _lib.require_cuda(codes, what)
+    _lib.require_cuda(scales, what)
     if not (codes.is_contiguous() and scales.is_contiguous() and codes.get_device() == scales.get_device()):
         raise ValueError(f"{what}: contiguous codes and scales on one device")
-    want = (torch.bfloat16, n) if kind == "pair" else (torch.float32, blocks(n))
-    if codes.dtype != _CODE_DTYPE[kind] or scales.dtype != want[0] or scales.numel() != want[1]:
-        raise ValueError(f"{what}: a {kind!r} state of {n} elements has {_CODE_DTYPE[kind]} codes and "
-                         f"{want[1]} {want[0]} scales (got {codes.dtype}, {scales.numel()} {scales.dtype})")
+    want = (torch.bfloat16, n) if pair else (torch.float32, blocks(n))
+    raise ValueError(f"{what}: a {kind!r} state of {n} elements has {_CODE_DTYPE[kind]} codes and "
+                     f"{want[1]} {want[0]} scales (got {codes.dtype}, {scales.numel()} {scales.dtype})")
 
 
 def check_state(p, codes, scales, kind, what):
@@ -79,21 +82,25 @@ def check_state(p, codes, scales, kind, what):
 
 
 class Rows:
-    """Descriptors of one call (b2o_state_tensor as 64-bit words), by device."""
+    """Descriptors of one call (b2o_state_tensor as 64-bit words), by device.
+    ``extend(index)`` gives the function that appends value pointer, codes
+    pointer, scales pointer, numel and kind | value code << 32."""
     __slots__ = ("by",)
 
     def __init__(self):
         self.by = {}
 
-    def add(self, value, codes, scales, n, kind, value_code):
-        words = self.by.get(value.get_device())
+    def extend(self, index):
+        words = self.by.get(index)
         if words is None:
-            words = self.by[value.get_device()] = array("Q")
-        words.extend((value.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, kind | value_code << 32))
+            words = self.by[index] = array("Q")
+        return words.extend
 
     def launch(self, fn, what):
         for index, words in self.by.items():
             n = len(words) // _WORDS
+            if not n:
+                continue
             dev = torch.device("cuda", index)
             with _lib.on_device(dev):
                 _lib.check(fn((_lib.StateTensor * n).from_buffer(words), n, _lib.stream_ptr(dev)), what)
@@ -103,19 +110,19 @@ class Rows:
 def encode(items):
     """[(tensor, kind), ...] -> [(codes, scales), ...] ("pair": (bf16 weight, bf16
     remainder)). ``tensor``: contiguous fp32 or bf16 CUDA tensor; codes keep its shape."""
-    out, rows = [], Rows()
+    out, rows, last, extend = [], Rows(), None, None
+    empty, empty_like, f32 = torch.empty, torch.empty_like, torch.float32
     for value, kind in items:
         code = _kind(kind)
         value_code = _value_code(value, "state8.encode")
-        n = value.numel()
-        codes = torch.empty_like(value, dtype=_CODE_DTYPE[kind])
-        if kind == "pair":
-            scales = torch.empty_like(codes)
-        else:
-            scales = torch.empty(blocks(n), dtype=torch.float32, device=value.device)
+        n, index = value.numel(), value.get_device()
+        codes = empty_like(value, dtype=_CODE_DTYPE[kind])
+        scales = empty_like(codes) if kind == "pair" else empty((n + BLOCK - 1) // BLOCK, dtype=f32, device=value.device)
         out.append((codes, scales))
         if n:
-            rows.add(value, codes, scales, n, code, value_code)
+            if index != last:
+                last, extend = index, rows.extend(index)
+            extend((value.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, code | value_code << 32))
     rows.launch(_lib.load().b2o_state_encode, "state_encode")
     return out
 
@@ -128,31 +135,35 @@ def decode(items, dtype=torch.float32, out=None):
     ``out``: contiguous tensors to write instead of new ones (their dtype counts);
     they may not overlap."""
     items = list(items)
-    if out is not None and len(out) != len(items):
-        raise ValueError(f"state8.decode: {len(items)} states and {len(out)} outputs")
+    if out is not None:
+        if len(out) != len(items):
+            raise ValueError(f"state8.decode: {len(items)} states and {len(out)} outputs")
+        at = [t.data_ptr() for t in out if t.numel()]
+        if len(set(at)) != len(at):
+            raise ValueError("state8.decode: an output appears twice")
     many = isinstance(dtype, (list, tuple))
     if many and len(dtype) != len(items):
         raise ValueError(f"state8.decode: {len(items)} states and {len(dtype)} dtypes")
-    if out is not None and len({t.data_ptr() for t in out if t.numel()}) != sum(1 for t in out if t.numel()):
-        raise ValueError("state8.decode: an output appears twice")
-    values, rows = [], Rows()
+    values, rows, last, extend, empty_like = [], Rows(), None, None, torch.empty_like
     for i, (codes, scales, kind) in enumerate(items):
         code = _kind(kind)
-        n = codes.numel()
+        n, index = codes.numel(), codes.get_device()
         _check_codes(codes, scales, kind, n, "state8.decode")
         if out is not None:
             value = out[i]
             value_code = _value_code(value, "state8.decode")
-            if value.numel() != n or value.get_device() != codes.get_device():
+            if value.numel() != n or value.get_device() != index:
                 raise ValueError("state8.decode: an output has its codes' size and device")
         else:
             dt = dtype[i] if many else dtype
             value_code = _VALUE_CODE.get(dt)
             if value_code is None:
                 raise TypeError(f"state8.decode: values are float32 or bfloat16 (got {dt})")
-            value = torch.empty_like(codes, dtype=dt)
+            value = empty_like(codes, dtype=dt)
         values.append(value)
         if n:
-            rows.add(value, codes, scales, n, code, value_code)
+            if index != last:
+                last, extend = index, rows.extend(index)
+            extend((value.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, code | value_code << 32))
     rows.launch(_lib.load().b2o_state_decode, "state_decode")
     return values

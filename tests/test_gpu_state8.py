@@ -514,6 +514,7 @@ def test_small_tensors_keep_wide_moments(cuda):
     for k in ("exp_avg", "exp_avg_sq", "mant_rem"):
         assert torch.equal(opt.state[small][k], wide.state[w][k])
     assert torch.equal(small, w)
+    assert torch.equal(wide.expanded_state()[0]["exp_avg_sq"], wide.state[w]["exp_avg_sq"])  # nothing to expand
     x = opt.expanded_state()
     assert torch.equal(x[1]["exp_avg"], wide.state[w]["exp_avg"])
     assert torch.equal(x[0]["master"], big.detach().float() + opt.state[big]["mant_rem"].float())
