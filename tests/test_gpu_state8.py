@@ -741,6 +741,43 @@ def test_expanded_checkpoint_has_the_reference_layout(cuda, tmp_path):
     _train(narrow[0], narrow[1], narrow[2], narrow[3], range(1))
 
 
+def test_the_ranks_of_a_sharded_step_give_the_whole_step(cuda):
+    """Each of two ranks' own part of a step (run one after the other, without the exchange) is the part of the
+    unsharded step, bit for bit: parameters, codes, scales, remainders, momenta."""
+    from sol_b200.sharding import ShardedStep
+    grads = [[g.cuda() for g in synth.make_grads(synth.SyntheticLM(synth.MICRO, seed=0), 0, 0)]]
+    whole = _setup()
+    ranks = []
+    for rank in range(2):
+        model, muon, adamw, ema = _setup()
+        sh = ShardedStep(model, muon, adamw, ema, 2, rank, min_rows_shard=16, exchange="nccl")
+        ranks.append((model, muon, adamw, sh))
+    assert any(adamw.holds_8bit(p) for p in ranks[0][3].row_sharded)
+    # one step: the next would need the weights and states that the ranks exchange
+    for model, muon, adamw, _ in [(whole[0], whole[1], whole[2], None)] + ranks:
+        synth.set_grads(model, [g.clone() for g in grads[0]])
+        adamw.step()
+        muon.step()
+    torch.cuda.synchronize()
+    for rank, (model, muon, adamw, sh) in enumerate(ranks):
+        pairs = list(zip([p for g in adamw.param_groups for p in g["params"]],
+                         [p for g in whole[2].param_groups for p in g["params"]]))
+        for p, q in pairs:
+            start, n = adamw._owned_slices[id(p)]
+            for k, v in {**whole[2].state[q], "p": q.detach()}.items():
+                w = adamw.state[p][k] if k != "p" else p.detach()
+                lo, hi = (start // 128, -(-(start + n) // 128)) if k.endswith("_scale") else (start, start + n)
+                if k == "step":
+                    lo, hi = 0, 1
+                assert torch.equal(w.reshape(-1)[lo:hi], v.reshape(-1)[lo:hi]), (rank, tuple(p.shape), k)
+        for p, q in zip([p for g in muon.param_groups for p in g["params"]], [p for g in whole[1].param_groups for p in g["params"]]):
+            if sh.owner[id(p)] == rank:
+                assert torch.equal(p, q)
+                for k, v in whole[1].state[q].items():
+                    w = muon.state[p][k]
+                    assert torch.equal(w, v) if torch.is_tensor(v) else w == v, (rank, k)
+
+
 # ---------------------------------------------------------- NorMuon momentum --
 def _front8(cuda, shapes, dtype, nesterov, steps, x0=False, coef=None, seed=0, beta=0.9, scale_of=lambda t: 1e-3):
     """Runs the front (and, with x0, the prescale) call over several steps and checks each against the restatement."""
