@@ -738,7 +738,7 @@ __device__ __forceinline__ void front8_tile(const Front8In<T, N>& in8, const Fro
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 y = f2_split(mul2(x.p[j], f2(a.kx)));
-        w[j] = f32_to_f16(y.x) | static_cast<uint32_t>(f32_to_f16(y.y)) << 16;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(y.y), "f"(y.x));
       }
       u.a = make_uint4(w[0], w[1], w[2], w[3]);
     }
