@@ -250,6 +250,14 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
                            "there is no CPU fallback")
 
 
+def require_match(t: torch.Tensor, p: torch.Tensor, numel: int, dtypes, what: str) -> None:
+    """Refuses a state tensor of parameter p that is not ``numel`` dense elements
+    of one of ``dtypes`` on p's device: the kernels take its pointer alone."""
+    if t.numel() != numel or t.dtype not in dtypes or t.get_device() != p.get_device() or not t.is_contiguous():
+        raise ValueError(f"{what}: {numel} contiguous elements of {' or '.join(map(str, dtypes))} on {p.device} for a "
+                         f"parameter of shape {tuple(p.shape)} (got {t.numel()} of {t.dtype} on {t.device})")
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

@@ -73,6 +73,7 @@ class AdamW(torch.optim.Optimizer):
         self._ema_weight = 0.0
         self._grad_scale = None    # device fp32 clip coefficient for the next step (clip_grad_norm_ defer_to)
         self._plan = None          # cached launch descriptors (see step)
+        self._checked = {}         # id(param) -> what expanded_state last found to fit it
         register_optimizer(self)
 
     @staticmethod
@@ -117,7 +118,7 @@ class AdamW(torch.optim.Optimizer):
         holds (on the GPU; needs the parameters there)."""
         from .normuon import _load_state_keep_dtypes
         _load_state_keep_dtypes(self, state_dict)
-        self._plan = None
+        self.invalidate_plan()
         self._convert_loaded()
         for group in self.param_groups:
             for p in group["params"]:
@@ -150,11 +151,23 @@ class AdamW(torch.optim.Optimizer):
                 [(st["exp_avg"], st.pop("exp_avg_scale"), "signed"),
                  (st["exp_avg_sq"], st.pop("exp_avg_sq_scale"), "root")], dtype=dt)
 
+    @staticmethod
+    def _check_narrow(p, st):
+        """Refuses 8-bit moments and a remainder that are not those of parameter p."""
+        m, v = st["exp_avg"], st["exp_avg_sq"]
+        if m.dtype == torch.int8 or v.dtype == torch.uint8:
+            state8.check_state(p, m, st.get("exp_avg_scale"), "signed", "AdamW: exp_avg")
+            state8.check_state(p, v, st.get("exp_avg_sq_scale"), "root", "AdamW: exp_avg_sq")
+        rem = st.get("mant_rem")
+        if rem is not None and p.dtype == torch.bfloat16:
+            _lib.require_match(rem, p, p.numel(), (torch.bfloat16,), "AdamW: mant_rem")
+
     @torch.no_grad()
     def expanded_state(self, params=None, dtype=torch.float32):
         """The moments as ``dtype`` (fp32 or bf16) tensors, and the fp32 master
         weight where a bf16 parameter has a remainder: one dict per parameter
-        with "exp_avg", "exp_avg_sq" and, there, "master". 8-bit moments and
+        with "exp_avg", "exp_avg_sq" and, there, "master". A state that does not
+        fit its parameter is refused. 8-bit moments and
         master weights of all parameters are expanded in one launch; moments
         that are wide already are cast by torch. (In a sharded step a rank's
         moments are those of its own rows until ``gather_state``.)"""
@@ -167,6 +180,7 @@ class AdamW(torch.optim.Optimizer):
         pair = 2 | _lib.F32 << 32
         out, rows, last, extend = [], state8.Rows(), None, None
         empty, eight, f32, states = torch.empty_like, torch.int8, torch.float32, self.state
+        checked, unseen = self._checked, (None,) * 9
         for p in params:
             index = p.get_device()
             if index != last:
@@ -176,16 +190,23 @@ class AdamW(torch.optim.Optimizer):
             if not st or "exp_avg" not in st:
                 st = self._init_state(p)
             m, v, n = st["exp_avg"], st["exp_avg_sq"], p.numel()
-            if m.dtype is eight:
+            get = st.get
+            ms, vs, rem = get("exp_avg_scale"), get("exp_avg_sq_scale"), get("mant_rem")
+            # The kernel takes n elements of each. The same tensors are looked over once.
+            m0, v0, ms0, vs0, rem0, n0, index0, narrow, pair_of = checked.get(id(p), unseen)
+            if not (m is m0 and v is v0 and ms is ms0 and vs is vs0 and rem is rem0 and n == n0 and index == index0):
+                self._check_narrow(p, st)
+                narrow, pair_of = m.dtype is eight, rem if p.dtype is torch.bfloat16 else None
+                checked[id(p)] = (m, v, ms, vs, rem, n, index, narrow, pair_of)
+            if narrow:
                 a, b = empty(m, dtype=dtype), empty(v, dtype=dtype)
                 if n:
-                    extend((a.data_ptr(), m.data_ptr(), st["exp_avg_scale"].data_ptr(), n, signed,
-                            b.data_ptr(), v.data_ptr(), st["exp_avg_sq_scale"].data_ptr(), n, root))
+                    extend((a.data_ptr(), m.data_ptr(), ms.data_ptr(), n, signed,
+                            b.data_ptr(), v.data_ptr(), vs.data_ptr(), n, root))
             else:
                 a, b = m.to(dtype, copy=True), v.to(dtype, copy=True)
             wide = {"exp_avg": a, "exp_avg_sq": b}
-            rem = st.get("mant_rem")
-            if rem is not None:
+            if pair_of is not None:
                 if not p.is_contiguous():
                     raise ValueError("AdamW.expanded_state: contiguous parameters only")
                 wide["master"] = w = empty(rem, dtype=f32)
@@ -200,7 +221,7 @@ class AdamW(torch.optim.Optimizer):
         sd = self.state_dict()
         for p, key in self._state_keys(sd):
             st = sd["state"].get(key)
-            if st and "exp_avg" in st and st["exp_avg"].dtype == torch.int8:
+            if st and "exp_avg" in st and (st["exp_avg"].dtype == torch.int8 or st["exp_avg_sq"].dtype == torch.uint8):
                 wide = self.expanded_state([p])[0]
                 sd["state"][key] = {k: wide.get(k, v) for k, v in st.items()
                                     if k not in ("exp_avg_scale", "exp_avg_sq_scale")}
@@ -217,6 +238,7 @@ class AdamW(torch.optim.Optimizer):
         parameters, moved parameter storage, gradients appearing or vanishing,
         EMA folding and shard changes themselves."""
         self._plan = None
+        self._checked = {}
 
     def _build_plan(self, ps, gis, key):
         """Launch descriptors for the parameters (with gradients) of this step:

@@ -59,6 +59,17 @@ def _value_code(t, what) -> int:
     return code
 
 
+def check_sizes(n, codes, scales, kind, what):
+    """Refuses codes and scales that are not those of a state of n elements: their
+    types and numbers, on whatever device."""
+    if scales is None:
+        raise ValueError(f"{what}: a {kind!r} state without scales")
+    want = (torch.bfloat16, n) if kind == "pair" else (torch.float32, blocks(n))
+    if (codes.dtype, codes.numel(), scales.dtype, scales.numel()) != (_CODE_DTYPE[kind], n, *want):
+        raise ValueError(f"{what}: a {kind!r} state of {n} elements has {n} {_CODE_DTYPE[kind]} codes and "
+                         f"{want[1]} {want[0]} scales (got {codes.numel()} {codes.dtype}, {scales.numel()} {scales.dtype})")
+
+
 def _check_codes(codes, scales, kind, n, what):
     pair = kind == "pair"
     if (codes.dtype is _CODE_DTYPE[kind] and scales.dtype is (torch.bfloat16 if pair else torch.float32) and
@@ -69,15 +80,15 @@ def _check_codes(codes, scales, kind, n, what):
     _lib.require_cuda(scales, what)
     if not (codes.is_contiguous() and scales.is_contiguous() and codes.get_device() == scales.get_device()):
         raise ValueError(f"{what}: contiguous codes and scales on one device")
-    want = (torch.bfloat16, n) if pair else (torch.float32, blocks(n))
-    raise ValueError(f"{what}: a {kind!r} state of {n} elements has {_CODE_DTYPE[kind]} codes and "
-                     f"{want[1]} {want[0]} scales (got {codes.dtype}, {scales.numel()} {scales.dtype})")
+    check_sizes(n, codes, scales, kind, what)
 
 
 def check_state(p, codes, scales, kind, what):
     """Refuses a state that does not belong to parameter p (a loaded one may not)."""
     if codes.numel() != p.numel() or codes.get_device() != p.get_device():
         raise ValueError(f"{what}: {codes.numel()} codes for a parameter of {p.numel()} elements, or on another device")
+    if scales is None:
+        raise ValueError(f"{what}: a {kind!r} state without scales")
     _check_codes(codes, scales, kind, p.numel(), what)
 
 
