@@ -272,11 +272,11 @@ class AdamW(torch.optim.Optimizer):
                     if sl is None:
                         continue
                     start, n = sl
+                self._check_narrow(p, st)
+                _lib.require_match(st["step"], p, 1, (torch.float32,), "AdamW: step")
                 esz = p.element_size()
                 ssz = st["exp_avg"].element_size()
                 if sdt == torch.int8:
-                    state8.check_state(p, st["exp_avg"], st["exp_avg_scale"], "signed", "AdamW: exp_avg")
-                    state8.check_state(p, st["exp_avg_sq"], st["exp_avg_sq_scale"], "root", "AdamW: exp_avg_sq")
                     if start % state8.BLOCK or ((start + n) % state8.BLOCK and start + n != p.numel()):
                         raise ValueError("AdamW: a slice of 8-bit moments starts and ends at multiples of "
                                          f"{state8.BLOCK} elements (got {start}, {n} of {p.numel()})")
@@ -294,6 +294,8 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     if st["exp_avg_sq"].dtype != sdt:
                         raise ValueError("AdamW: exp_avg and exp_avg_sq of one dtype (or both in 8 bits)")
+                    for k in ("exp_avg", "exp_avg_sq"):
+                        _lib.require_match(st[k], p, p.numel(), (sdt,), f"AdamW: {k}")
                     descs.append(_lib.AdamwTensor(
                         p.data_ptr() + start * esz,
                         (rem.data_ptr() + start * 2) if rem is not None else None,

@@ -111,3 +111,38 @@ def test_a_remainder_beside_an_fp32_parameter_is_not_expanded(host):
     p, opt = _adamw(dtype=torch.float32)
     opt._init_state(p)["mant_rem"] = torch.zeros(64, 128, dtype=torch.bfloat16)
     assert set(opt.expanded_state()[0]) == {"exp_avg", "exp_avg_sq"}
+
+
+# ----------------------------------------------------------------- AdamW.step --
+def test_a_step_on_states_that_fit_is_launched(host):
+    for dt in (torch.int8, torch.float32, torch.bfloat16):
+        p, opt = _adamw(state_dtype=dt)
+        opt.step()
+        opt.step()
+    assert host.calls == ["b2o_adamw8_step"] * 2 + ["b2o_adamw_step"] * 4
+
+
+@pytest.mark.parametrize("key,change", BAD_ADAMW + [("step", lambda t: t.double()), ("step", lambda t: t.expand(2))])
+def test_adamw_step_refuses_a_state_that_does_not_fit(host, key, change):
+    p, opt = _adamw()
+    opt._init_state(p)
+    bad = change(opt.state[p][key])
+    if bad is None:
+        del opt.state[p][key]
+    else:
+        opt.state[p][key] = bad
+    with pytest.raises(ValueError, match=key.replace("_scale", "")):
+        opt.step()
+    assert host.calls == []
+
+
+@pytest.mark.parametrize("key,change", [("exp_avg", _cut), ("exp_avg_sq", _cut), ("mant_rem", _cut),
+                                        ("exp_avg_sq", lambda t: t.bfloat16()), ("mant_rem", lambda t: t.float()),
+                                        ("exp_avg", lambda t: t.t().contiguous().t()), ("step", lambda t: t.double())])
+def test_adamw_step_refuses_a_wide_state_that_does_not_fit(host, key, change):
+    p, opt = _adamw(state_dtype=torch.float32)
+    opt._init_state(p)
+    opt.state[p][key] = change(opt.state[p][key])
+    with pytest.raises(ValueError, match=key):
+        opt.step()
+    assert host.calls == []
