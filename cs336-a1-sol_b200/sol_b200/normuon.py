@@ -232,6 +232,17 @@ class NorMuonGNS(torch.optim.Optimizer):
             st["mant_rem"] = torch.zeros_like(p)
         return st
 
+    def _check_state(self, p, st):
+        """Refuses a state that does not belong to parameter p (a loaded one may not)."""
+        if self.momentum_dtype is not None:
+            state8.check_state(p, st["momentum_buffer"], st.get("momentum_scale"), "signed",
+                               "NorMuonGNS: momentum_buffer")
+        else:
+            _lib.require_match(st["momentum_buffer"], p, p.numel(), (p.dtype,), "NorMuonGNS: momentum_buffer")
+        _lib.require_match(st["v_row"], p, p.shape[0], (torch.float32,), "NorMuonGNS: v_row")
+        if self.bf16_master and p.dtype == torch.bfloat16:
+            _lib.require_match(st["mant_rem"], p, p.numel(), (torch.bfloat16,), "NorMuonGNS: mant_rem")
+
     def _prepare(self, params, shape, group):
         """Validates one exact-shape batch and returns its record (state, workspace)."""
         p0 = params[0]
@@ -245,6 +256,8 @@ class NorMuonGNS(torch.optim.Optimizer):
             if p.grad.dtype != p.dtype or not p.is_contiguous() or not p.grad.is_contiguous():
                 raise ValueError("NorMuonGNS needs contiguous params and grads of the param dtype")
         states = [self._init_state(p) for p in params]
+        for p, st in zip(params, states):
+            self._check_state(p, st)
         ws = self._workspace(dev, S, r, c)
         m, n = min(r, c), max(r, c)
         # the front writes the Gram iteration's binary16 input directly unless
@@ -276,9 +289,6 @@ class NorMuonGNS(torch.optim.Optimizer):
         keeps them alive."""
         if self.momentum_dtype is None:
             return None
-        for b in members:
-            for p, st in zip(b["params"], b["states"]):
-                state8.check_state(p, st["momentum_buffer"], st["momentum_scale"], "signed", "NorMuonGNS: momentum_buffer")
         scales = [_lib.ptr_array([st["momentum_scale"].data_ptr() for st in b["states"]]) for b in members]
         steps = [np.zeros(b["S"], dtype=np.uint32) for b in members]
         return (_lib.ptr_array([_lib.addr(x) for x in scales]), _lib.ptr_array([x.ctypes.data for x in steps]),

@@ -146,3 +146,44 @@ def test_adamw_step_refuses_a_wide_state_that_does_not_fit(host, key, change):
     with pytest.raises(ValueError, match=key):
         opt.step()
     assert host.calls == []
+
+
+# ------------------------------------------------------------ NorMuonGNS.step --
+def _muon(**kw):
+    p = torch.nn.Parameter(torch.zeros(64, 128, dtype=torch.bfloat16))
+    p.grad = torch.ones_like(p)
+    return p, NorMuonGNS([p], bf16_master=True, **kw)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(momentum_dtype=torch.int8)])
+@pytest.mark.parametrize("hooked", [False, True])
+def test_a_muon_step_on_states_that_fit_is_launched(host, kw, hooked):
+    p, opt = _muon(**kw)
+    if hooked:
+        opt._orthogonalize_batch = lambda U, n: torch.zeros_like(U)
+    opt.step()
+    opt.step()
+    assert sum("front" in c for c in host.calls) == 2 and sum("apply" in c for c in host.calls) == 2
+
+
+@pytest.mark.parametrize("kw,key,change", [
+    ({}, "momentum_buffer", _cut), ({}, "momentum_buffer", lambda t: t.float()), ({}, "momentum_buffer", lambda t: t.to(torch.int8)),
+    ({}, "v_row", _cut), ({}, "v_row", lambda t: t.bfloat16()), ({}, "mant_rem", _cut), ({}, "mant_rem", lambda t: t.float()),
+    ({}, "mant_rem", lambda t: t.t().contiguous().t()),
+    (dict(momentum_dtype=torch.int8), "momentum_buffer", _cut), (dict(momentum_dtype=torch.int8), "momentum_scale", _cut),
+    (dict(momentum_dtype=torch.int8), "momentum_scale", lambda t: None),
+    (dict(momentum_dtype=torch.int8), "momentum_buffer", lambda t: t.float()), (dict(momentum_dtype=torch.int8), "v_row", _cut)])
+@pytest.mark.parametrize("hooked", [False, True])
+def test_muon_step_refuses_a_state_that_does_not_fit(host, kw, key, change, hooked):
+    p, opt = _muon(**kw)
+    if hooked:
+        opt._orthogonalize_batch = lambda U, n: torch.zeros_like(U)
+    opt._init_state(p)
+    bad = change(opt.state[p][key])
+    if bad is None:
+        del opt.state[p][key]
+    else:
+        opt.state[p][key] = bad
+    with pytest.raises(ValueError, match=key.replace("scale", "buffer")):
+        opt.step()
+    assert host.calls == []
