@@ -115,16 +115,33 @@ class AdamW(torch.optim.Optimizer):
         """Keeps each saved state tensor's dtype (fp32 moments of bf16 parameters
         in master mode; torch's loader would cast them to bf16), except between
         8-bit and wider moments: those are converted to what this optimizer
-        holds (on the GPU; needs the parameters there)."""
+        holds (on the GPU; needs the parameters there). A state that does not
+        fit its parameter is refused, and nothing is loaded."""
         from .normuon import _load_state_keep_dtypes
-        _load_state_keep_dtypes(self, state_dict)
+        _load_state_keep_dtypes(self, state_dict, self._check_loaded)
         self.invalidate_plan()
         self._convert_loaded()
         for group in self.param_groups:
             for p in group["params"]:
                 st = self.state.get(p)
                 if st and "step" in st:
+                    st["step"] = st["step"].float()
                     self._steps[id(p)] = int(float(st["step"].item()))
+
+    @staticmethod
+    def _check_loaded(p, st):
+        from .normuon import _check_loaded_size
+        n, m, v = p.numel(), st.get("exp_avg"), st.get("exp_avg_sq")
+        if m is not None and v is not None and (m.dtype == torch.int8 or v.dtype == torch.uint8):
+            state8.check_sizes(n, m, st.get("exp_avg_scale"), "signed", "AdamW: the loaded exp_avg")
+            state8.check_sizes(n, v, st.get("exp_avg_sq_scale"), "root", "AdamW: the loaded exp_avg_sq")
+        else:
+            _check_loaded_size(st, "exp_avg", n, None, "AdamW")
+            _check_loaded_size(st, "exp_avg_sq", n, None, "AdamW")
+        if p.dtype == torch.bfloat16:
+            _check_loaded_size(st, "mant_rem", n, (torch.bfloat16,), "AdamW")
+        if torch.is_tensor(st.get("step")):
+            _check_loaded_size(st, "step", 1, None, "AdamW")
 
     def _convert_loaded(self):
         narrow, widen = [], []

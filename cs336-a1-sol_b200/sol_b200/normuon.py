@@ -34,16 +34,29 @@ from .polar_express import table_for
 MAX_BATCH = 64  # matrices per launch (kernel-parameter tables)
 
 
-def _load_state_keep_dtypes(opt, state_dict):
+def _load_state_keep_dtypes(opt, state_dict, check):
     """torch.optim.Optimizer.load_state_dict without the cast of floating-point
-    state to the parameter dtype: tensors move to the parameter's device only."""
+    state to the parameter dtype: tensors move to the parameter's device only
+    (dense, as the kernels take them). ``check(p, state)`` refuses a state that
+    does not belong to parameter p; the optimizer is then left as it was."""
     saved = state_dict["state"]
+    params = [p for g in opt.param_groups for p in g["params"]]
+    for idx, st in saved.items():
+        if int(idx) < len(params):  # (else torch refuses the groups)
+            check(params[int(idx)], st)
     torch.optim.Optimizer.load_state_dict(opt, {"state": {}, "param_groups": state_dict["param_groups"]})
     params = [p for g in opt.param_groups for p in g["params"]]
     for idx, st in saved.items():
         p = params[int(idx)]
-        opt.state[p] = {k: (v.detach().to(device=p.device).clone() if torch.is_tensor(v) else v)
-                        for k, v in st.items()}
+        opt.state[p] = {k: (v.detach().to(device=p.device).clone(memory_format=torch.contiguous_format)
+                            if torch.is_tensor(v) else v) for k, v in st.items()}
+
+
+def _check_loaded_size(st, key, numel, dtypes, what):
+    t = st.get(key)
+    if t is not None and (t.numel() != numel or not (t.dtype in dtypes if dtypes else t.dtype.is_floating_point)):
+        raise ValueError(f"{what}: the loaded {key} has {t.numel()} elements of {t.dtype} where the parameter's has "
+                         f"{numel} of {' or '.join(map(str, dtypes)) if dtypes else 'a floating-point type'}")
 
 
 class NorMuonGNS(torch.optim.Optimizer):
@@ -171,10 +184,24 @@ class NorMuonGNS(torch.optim.Optimizer):
         parameter dtype, which would turn the fp32 v_row of bf16 matrices into
         bf16), except between an 8-bit momentum and a wide one: those are
         converted to what this optimizer holds (on the GPU; needs the parameters
-        there)."""
-        _load_state_keep_dtypes(self, state_dict)
+        there). A wide momentum is cast to the parameter dtype and v_row to fp32,
+        the types that the kernels read. A state that does not fit its parameter
+        is refused, and nothing is loaded."""
+        _load_state_keep_dtypes(self, state_dict, self._check_loaded)
         self._plans = {}
         self._convert_loaded()
+
+    @staticmethod
+    def _check_loaded(p, st):
+        m = st.get("momentum_buffer")
+        if m is not None and m.dtype == torch.int8:
+            state8.check_sizes(p.numel(), m, st.get("momentum_scale"), "signed", "NorMuonGNS: the loaded momentum_buffer")
+        else:
+            _check_loaded_size(st, "momentum_buffer", p.numel(), None, "NorMuonGNS")
+        if p.dim() == 2:
+            _check_loaded_size(st, "v_row", p.shape[0], None, "NorMuonGNS")
+        if p.dtype == torch.bfloat16:
+            _check_loaded_size(st, "mant_rem", p.numel(), (torch.bfloat16,), "NorMuonGNS")
 
     def _convert_loaded(self):
         narrow, widen = [], []
@@ -183,6 +210,10 @@ class NorMuonGNS(torch.optim.Optimizer):
                 st = self.state.get(p)
                 if not st or "momentum_buffer" not in st:
                     continue
+                if "v_row" in st:
+                    st["v_row"] = st["v_row"].float()
+                if self.momentum_dtype is None and st["momentum_buffer"].dtype != torch.int8:
+                    st["momentum_buffer"] = st["momentum_buffer"].to(p.dtype)
                 eight = st["momentum_buffer"].dtype == torch.int8
                 if self.momentum_dtype == torch.int8 and not eight:
                     narrow.append(st)

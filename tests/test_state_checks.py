@@ -187,3 +187,92 @@ def test_muon_step_refuses_a_state_that_does_not_fit(host, kw, key, change, hook
     with pytest.raises(ValueError, match=key.replace("scale", "buffer")):
         opt.step()
     assert host.calls == []
+
+
+# -------------------------------------------------------------------- loading --
+def _saved(opt, p, step=3.0):
+    st = opt._init_state(p)
+    if "step" in st:
+        st["step"].fill_(step)
+    return opt.state_dict()
+
+
+def _snapshot(opt):
+    return {k: {n: (t, t._version) if torch.is_tensor(t) else t for n, t in st.items()} for k, st in opt.state.items()}
+
+
+def _same(a, b):
+    """The same states, and each value the same tensor (and not written), or equal."""
+    return set(map(id, a)) == set(map(id, b)) and all(
+        set(a[p]) == set(b[p]) and all(x[0] is y[0] and x[1] == y[1] if isinstance(x, tuple) else x == y
+                                       for x, y in ((a[p][n], b[p][n]) for n in a[p])) for p in a)
+
+
+@pytest.mark.parametrize("make,kw", [(_adamw, {}), (_adamw, dict(state_dtype=torch.float32)), (_muon, {}),
+                                     (_muon, dict(momentum_dtype=torch.int8))])
+@pytest.mark.parametrize("shape", [(32, 128), (128, 128), (64, 130)])
+def test_a_state_of_another_parameter_is_not_loaded(host, make, kw, shape):
+    """Before, the state of a 32 x 128 tensor loaded into an optimizer over 64 x 128."""
+    p, opt = make(**kw)
+    opt._init_state(p)
+    before, groups = _snapshot(opt), opt.state_dict()["param_groups"]
+    q = torch.nn.Parameter(torch.zeros(shape, dtype=torch.bfloat16))
+    other = AdamW([q], master="bf16_mt", lr=0.5, **{"state_dtype": torch.int8, **kw}) if make is _adamw else \
+        NorMuonGNS([q], bf16_master=True, lr=0.5, **kw)
+    with pytest.raises(ValueError, match="loaded"):
+        opt.load_state_dict(_saved(other, q))
+    assert _same(before, _snapshot(opt)) and opt.state_dict()["param_groups"] == groups
+
+
+@pytest.mark.parametrize("make,kw,bad", [(_adamw, {}, BAD_ADAMW[:10] + [("step", lambda t: torch.zeros(2))]),
+                                         (_adamw, dict(state_dtype=torch.float32),
+                                          [(k, _cut) for k in ("exp_avg", "exp_avg_sq", "mant_rem")] +
+                                          [("exp_avg", lambda t: t.to(torch.int16)), ("mant_rem", lambda t: t.to(torch.int8))]),
+                                         (_muon, {}, [(k, _cut) for k in ("momentum_buffer", "v_row", "mant_rem")] +
+                                          [("mant_rem", lambda t: t.float())]),
+                                         (_muon, dict(momentum_dtype=torch.int8),
+                                          [(k, _cut) for k in ("momentum_buffer", "momentum_scale", "v_row", "mant_rem")] +
+                                          [("momentum_scale", lambda t: None), ("momentum_scale", lambda t: t.bfloat16())])])
+def test_each_part_of_a_loaded_state_is_checked(host, make, kw, bad):
+    for key, change in bad:
+        p, opt = make(**kw)
+        sd = _saved(opt, p)
+        x = change(sd["state"][0][key])
+        sd["state"][0] = {k: v for k, v in {**sd["state"][0], key: x}.items() if v is not None}
+        before = _snapshot(opt)
+        with pytest.raises(ValueError, match="|".join(("loaded", "without scales"))):
+            opt.load_state_dict(sd)
+        assert _same(before, _snapshot(opt)), key
+
+
+@pytest.mark.parametrize("make,kw", [(_adamw, {}), (_adamw, dict(state_dtype=torch.float32)), (_muon, {}),
+                                     (_muon, dict(momentum_dtype=torch.int8))])
+def test_a_state_that_fits_is_loaded_and_steps(host, make, kw):
+    p, opt = make(**kw)
+    sd = _saved(opt, p)
+    opt.load_state_dict(sd)
+    opt.step()
+    assert host.calls and (make is _muon or opt._steps[id(p)] == 4)
+    with pytest.raises(ValueError, match="group"):  # torch's own refusal keeps its form
+        opt.load_state_dict({"state": {5: sd["state"][0]}, "param_groups": sd["param_groups"] * 2})
+
+
+def test_loaded_types_become_those_that_the_kernels_read(host):
+    """torch's loader in the reference leaves v_row in bf16 when a run is resumed, and a state saved from a transposed
+    parameter keeps its strides."""
+    p, opt = _muon()
+    st = opt._init_state(p)
+    x = torch.arange(64 * 128).view(64, 128).float() / 64
+    sd = {"state": {0: {"momentum_buffer": x.clone(), "v_row": torch.full((64, 1), 0.5, dtype=torch.bfloat16),
+                        "mant_rem": x.bfloat16().t().contiguous().t()}}, "param_groups": opt.state_dict()["param_groups"]}
+    opt.load_state_dict(sd)
+    st = opt.state[p]
+    assert st["v_row"].dtype == torch.float32 and st["momentum_buffer"].dtype == torch.bfloat16
+    assert torch.equal(st["momentum_buffer"], x.bfloat16()) and torch.equal(st["mant_rem"], x.bfloat16())
+    opt.step()
+    q, adam = _adamw(state_dtype=torch.float32)
+    sd = _saved(adam, q)
+    sd["state"][0] = {**sd["state"][0], "step": torch.tensor(3.0, dtype=torch.float64), "exp_avg": x.t().contiguous().t()}
+    adam.load_state_dict(sd)
+    assert torch.equal(adam.state[q]["exp_avg"], x) and adam._steps[id(q)] == 3
+    adam.step()
