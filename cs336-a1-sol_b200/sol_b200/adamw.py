@@ -289,6 +289,8 @@ class AdamW(torch.optim.Optimizer):
                     if sl is None:
                         continue
                     start, n = sl
+                if sdt != torch.int8 and st["exp_avg_sq"].dtype != sdt:
+                    raise ValueError("AdamW: exp_avg and exp_avg_sq of one dtype (or both in 8 bits)")
                 self._check_narrow(p, st)
                 _lib.require_match(st["step"], p, 1, (torch.float32,), "AdamW: step")
                 esz = p.element_size()
@@ -309,8 +311,6 @@ class AdamW(torch.optim.Optimizer):
                         (shadow.data_ptr() + start * 4) if shadow is not None else None,
                         n, start, gi, 0, st["step"].data_ptr()))
                 else:
-                    if st["exp_avg_sq"].dtype != sdt:
-                        raise ValueError("AdamW: exp_avg and exp_avg_sq of one dtype (or both in 8 bits)")
                     for k in ("exp_avg", "exp_avg_sq"):
                         _lib.require_match(st[k], p, p.numel(), (sdt,), f"AdamW: {k}")
                     descs.append(_lib.AdamwTensor(

@@ -136,6 +136,15 @@ def test_adamw_step_refuses_a_state_that_does_not_fit(host, key, change):
     assert host.calls == []
 
 
+def test_adamw_step_refuses_one_wide_moment_beside_8_bits(host):
+    p, opt = _adamw()
+    st = opt._init_state(p)
+    st["exp_avg"] = st["exp_avg"].float()
+    with pytest.raises(ValueError, match="one dtype"):
+        opt.step()
+    assert host.calls == []
+
+
 @pytest.mark.parametrize("key,change", [("exp_avg", _cut), ("exp_avg_sq", _cut), ("mant_rem", _cut),
                                         ("exp_avg_sq", lambda t: t.bfloat16()), ("mant_rem", lambda t: t.float()),
                                         ("exp_avg", lambda t: t.t().contiguous().t()), ("step", lambda t: t.double())])
