@@ -36,8 +36,9 @@ struct Adam8Coef {
   float one;                      // 1 (see mul_add2)
   float far;                      // a root whose denominator is finite and has the reciprocal 0
   int wd_on, cautious;
-  // 1: the roots of subnormal second moments may read as 0 in the update (eps
-  // covers them 2^24 times); 0: they are computed, and the division is IEEE's
+  // 1: the roots of subnormal second moments may read as anything below 2^-63 in
+  // the update (eps is more than 2^25 times that, so the denominator rounds to
+  // eps); 0: they are computed, and root and quotient are IEEE's
   int plain_roots;
   const float* grad_scale;
 };
@@ -64,7 +65,7 @@ __device__ __forceinline__ int find_tensor(const Table& tab, int chunk) {
 // One warp step: 256 elements, 8 a lane, blocks of 16 lanes.
 // FULL: all of them exist and every pointer takes vector accesses. EXTRA 1: a
 // group may have a clip coefficient or weight decay; 2: also an eps that does not
-// cover the roots of subnormal second moments (see plain_roots).
+// cover the roots of subnormal second moments (see plain_roots): a launch of its own.
 // `mine` are the step's first inputs, loaded during the step before.
 template <typename PT>
 struct Adam8In {
@@ -118,6 +119,7 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
   for (int j = 0; j < 4; ++j) {
     const float2 x = f2_split(v.p[j]);
     if (EXTRA < 2) r.p[j] = f2(sqrt_approx_ftz(x.x), sqrt_approx_ftz(x.y));
+    else if (REM) r.p[j] = f2(__fsqrt_rn(x.x), __fsqrt_rn(x.y));
     else r.p[j] = f2(sqrt_approx(x.x), sqrt_approx(x.y));
     if (REM && EXTRA < 2) {
       const F2 inv = f2(fminf(rsqrt_approx_ftz(x.x), 9.2233720e18f), fminf(rsqrt_approx_ftz(x.y), 9.2233720e18f));
@@ -288,7 +290,8 @@ int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8
     c.far = 3e38f / c.inv_bc2;
     c.wd_on = g.weight_decay != 0.0;
     c.cautious = g.cautious;
-    c.plain_roots = c.eps * 5.9604645e-8f >= 1.0842022e-19f * c.inv_bc2;  // eps 2^-24 >= 2^-63 inv_bc2
+    // eps 2^-25 >= 2^-63 inv_bc2 (and below the numbers whose reciprocal is subnormal)
+    c.plain_roots = c.eps * 2.9802322e-8f >= 1.0842022e-19f * c.inv_bc2 && c.eps < 1e37f;
     c.grad_scale = g.grad_scale;
   }
   tab.ema_weight = ema_weight;
@@ -303,24 +306,25 @@ int adamw8_step(const b2o_adamw8_tensor* tensors, int ntensors, const b2o_adamw8
     if (t.rem && param_dtype != B2O_BF16) { set_error("adamw8: remainder needs bf16 params"); return -1; }
     if ((t.numel + kS8Chunk - 1) / kS8Chunk > (1ll << 30)) { set_error("adamw8: tensor too large"); return -1; }
   }
-  // One launch for each mix of remainder and EMA (one in all, as a rule): the
-  // passes without them are then without their branches too.
-  for (int mix = 0; mix < 4; ++mix) {
-    const bool rem = (mix & 1) != 0, ema = (mix & 2) != 0;
+  // One launch for each mix of remainder, EMA and eps (one in all, as a rule): the
+  // passes without them are then without their branches too, and a tensor's
+  // result depends on its own group alone, not on what shares its launch.
+  for (int mix = 0; mix < 8; ++mix) {
+    const bool rem = (mix & 1) != 0, ema = (mix & 2) != 0, exact = (mix & 4) != 0;
     for (int at = 0; at < ntensors;) {
       int n = 0, chunks = 0;
       int extra = 0;
       for (; at < ntensors && n < kS8Tensors; ++at) {
         const b2o_adamw8_tensor& t = tensors[at];
-        if (t.numel == 0 || (t.rem != nullptr) != rem || (t.ema != nullptr) != ema) continue;
+        const Adam8Coef& c = tab.g[t.group];
+        if (t.numel == 0 || (t.rem != nullptr) != rem || (t.ema != nullptr) != ema || (c.plain_roots == 0) != exact) continue;
         const int ch = static_cast<int>((t.numel + kS8Chunk - 1) / kS8Chunk);
         if (n > 0 && chunks + static_cast<int64_t>(ch) > (1ll << 30)) break;
         tab.t[n] = t;
         tab.chunk_start[n] = chunks;
         tab.vec_ok[n] = aligned16(t.param) && aligned16(t.grad) && aligned8(t.exp_avg) && aligned8(t.exp_avg_sq) &&
                         (!t.rem || aligned16(t.rem)) && (!t.ema || aligned16(t.ema));
-        const Adam8Coef& c = tab.g[t.group];
-        extra = std::max(extra, !c.plain_roots ? 2 : c.grad_scale || c.wd_on ? 1 : 0);
+        extra = std::max(extra, exact ? 2 : c.grad_scale || c.wd_on ? 1 : 0);
         chunks += ch;
         ++n;
       }

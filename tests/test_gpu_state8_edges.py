@@ -78,3 +78,84 @@ def test_a_gradient_that_is_not_finite_makes_its_weight_nan(cuda, dtype, master)
         p.grad[300] = bad
         opt.step()
         assert torch.equal(p.detach().isnan().nonzero().flatten().cpu(), torch.tensor([300]))
+
+
+# ----------------------------- an eps that does not cover the smallest roots --
+def _state(n):
+    return {"exp_avg": torch.zeros(n, dtype=torch.int8), "exp_avg_sq": torch.zeros(n, dtype=torch.uint8),
+            "exp_avg_scale": torch.zeros(state8.blocks(n)), "exp_avg_sq_scale": torch.zeros(state8.blocks(n))}
+
+
+@pytest.mark.parametrize("dtype,master", FORMS)
+@pytest.mark.parametrize("wd,cautious,ema,clip", [(0.0, False, False, None), (0.1, False, True, None), (0.1, True, False, 0.37),
+                                                  (0.0, False, True, 0.37)])
+@pytest.mark.parametrize("eps", [0.0, 1e-13])
+def test_a_tiny_eps_matches_the_restatement(cuda, dtype, master, wd, cautious, ema, clip, eps):
+    """Tolerance: codes and scales equal. The update: m and v each carry at most four roundings of 2^-24 of the sum of
+    their positive parts, root, quotient, products and coefficients fewer than 24 more, doubled: 64 x 2^-24 of the
+    update with nothing cancelled; decay and the sum 4 x 2^-24 of the weight; then the stored type: half a step, or
+    2^-16 with a remainder."""
+    n = 8192 + 999
+    cpu = (torch.randn(n, generator=_gen(2)) * 0.02).to(dtype)
+    p = torch.nn.Parameter(cpu.cuda())
+    opt = _optimizer([p], master=master, eps=eps, weight_decay=wd, cautious_wd=cautious)
+    avg = None
+    if ema:
+        avg = EmaWeights(torch.nn.ParameterList([p]), 0.999)
+        avg.update()
+    st = _state(n)
+    coef = None if clip is None else torch.tensor(clip, device=cuda)
+    for step in range(1, 4):
+        x = torch.randn(n, generator=_gen(100 + step)) * torch.exp(2 * torch.randn(n, generator=_gen(200 + step))) * 1e-3
+        x[::7] = torch.where(x[::7] < 0, -1e-18, 1e-18)  # squares below every eps here
+        x = x.to(dtype)
+        p0, rem = p.detach().cpu(), opt.state[p]["mant_rem"].cpu() if "mant_rem" in opt.state[p] else None
+        shadow = avg.shadow[0].cpu() if ema else None
+        if rem is None and master == "bf16_mt":
+            rem = torch.zeros_like(p0)
+        p.grad = x.cuda()
+        opt._grad_scale = coef
+        opt.step()
+        if ema:
+            avg.update()
+        if clip is not None:
+            x = (x.float() * torch.tensor(clip)).to(dtype)
+        m0 = ref.decode(st["exp_avg"], st["exp_avg_scale"], False).double().abs()
+        v0 = ref.decode(st["exp_avg_sq"], st["exp_avg_sq_scale"], True).double()
+        w = ref.adamw_step(p0, rem, x, st, lr=1.2e-2, betas=(0.9, 0.95), eps=eps, wd=wd, cautious=cautious, step=step)
+        for k in KEYS:
+            assert torch.equal(opt.state[p][k].cpu(), st[k]), (k, step)
+        a, v = 0.9 * m0 + 0.1 * x.double().abs(), 0.95 * v0 + 0.05 * x.double() ** 2
+        up = 1.2e-2 / (1 - 0.9 ** step) * a / (v.sqrt() / math.sqrt(1 - 0.95 ** step) + eps)
+        tol = 64 * 2.0 ** -24 * up + 4 * 2.0 ** -24 * (p0.double().abs() + w.abs()) + 1e-42
+        got = p.detach().cpu()
+        whole = got.double() + opt.state[p]["mant_rem"].cpu().double() if master == "bf16_mt" else got.double()
+        half = 2.0 ** -16 if master == "bf16_mt" else torch.finfo(dtype).eps / 2
+        # a second moment that is subnormal in fp32 (below 1e-38) keeps fewer bits than the tolerance counts
+        held = v > 1e-36
+        assert held.float().mean() > 0.8 and ((whole - w).abs() <= tol + half * (w.abs() + tol))[held].all(), step
+        if ema:
+            want = shadow.double() + (1.0 - 0.999) * (got.double() - shadow.double())
+            assert ((avg.shadow[0].cpu().double() - want).abs() <= 4 * 2.0 ** -24 * (shadow.abs() + got.float().abs())).all()
+
+
+@pytest.mark.parametrize("dtype,master", FORMS)
+def test_a_tensors_step_does_not_depend_on_what_shares_its_call(cuda, dtype, master):
+    """Groups with eps 1e-8 give the same bits alone and beside groups whose eps is 0 or tiny, decayed or not."""
+    n = 3 * 8192 + 77
+    def params(k):
+        # weights of 0: the update's last places stand in the stored bits
+        return [torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=cuda)) for _ in range(k)]
+    mixed, alone = params(4), params(4)
+    groups = [dict(eps=1e-8), dict(eps=0.0), dict(eps=1e-8, weight_decay=0.1), dict(eps=1e-14, weight_decay=0.1)]
+    opts = [_optimizer([{"params": [p], **g} for p, g in zip(mixed, groups)], master=master)]
+    opts += [_optimizer([{"params": [p], **g}], master=master) for p, g in zip(alone, groups)]
+    for step in range(1, 6):
+        for k, (p, q) in enumerate(zip(mixed, alone)):
+            p.grad = ((torch.randn(n, generator=_gen(10 * step + k)) + 0.01) * 1e-3).to(dtype).cuda()
+            q.grad = p.grad.clone()
+        for o in opts:
+            o.step()
+    for k, (p, q, o) in enumerate(zip(mixed, alone, opts[1:])):
+        assert torch.equal(p, q), k
+        assert all(torch.equal(opts[0].state[p][x], o.state[q][x]) for x in o.state[q]), k
