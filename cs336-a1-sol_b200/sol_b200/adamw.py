@@ -399,11 +399,7 @@ class AdamW(torch.optim.Optimizer):
         gptr = np.fromiter((g.data_ptr() for g in gs_), dtype=np.uint64, count=len(gs_))
         for words, where, offs in plan["refresh"]:
             words[:] = gptr[where] + offs
-        steps_of = {}
-        for gi, ids in plan["groups"].items():
-            k = self._steps.get(ids[0], 0) + 1
-            self._steps.update(dict.fromkeys(ids, k))
-            steps_of[gi] = k
+        steps_of = {gi: self._steps.get(ids[0], 0) + 1 for gi, ids in plan["groups"].items()}
         gsc = self._grad_scale.data_ptr() if self._grad_scale is not None else None
         groups = groups8 = None
         ngroups = len(self.param_groups)
@@ -419,6 +415,8 @@ class AdamW(torch.optim.Optimizer):
                         groups = self._groups(steps_of, gsc)
                     rc = lib.b2o_adamw_step(arr, n, groups, ngroups, pdt, sdt, self._ema_weight, _lib.stream_ptr(dev))
                     _lib.check(rc, "adamw_step")
+        for gi, ids in plan["groups"].items():  # a refused call leaves them
+            self._steps.update(dict.fromkeys(ids, steps_of[gi]))
         if self._ema is not None and plan["ema_idx"]:
             self._ema._folded |= plan["ema_idx"]
         self._grad_scale = None

@@ -85,9 +85,9 @@ class NorMuonGNS(torch.optim.Optimizer):
             raise ValueError("orthogonalizer must be 'gram' or 'quintic'")
         if momentum_dtype not in (None, torch.int8):
             raise ValueError("momentum_dtype must be None or torch.int8")
-        if momentum_dtype == torch.int8 and not all(0.0 <= g["momentum"] < 1.0 for g in self.param_groups):
-            raise ValueError("NorMuonGNS with an 8-bit momentum needs momentum in [0, 1)")
         self.momentum_dtype = momentum_dtype
+        for group in self.param_groups:
+            self._check_8bit_group(group)
         self.cautious_wd = cautious_wd
         self.bf16_master = bf16_master
         self.orthogonalizer = orthogonalizer
@@ -107,6 +107,10 @@ class NorMuonGNS(torch.optim.Optimizer):
         self._grad_scale = None    # device fp32 clip coefficient for the next step (clip_grad_norm_ defer_to)
         self._plans = {}           # (param-group index, owned set) -> cached launch descriptors (see step)
         register_optimizer(self)
+
+    def _check_8bit_group(self, group):
+        if self.momentum_dtype == torch.int8 and not 0.0 <= group["momentum"] < 1.0:
+            raise ValueError("NorMuonGNS with an 8-bit momentum needs momentum in [0, 1)")
 
     # ------------------------------------------------------------------ hooks
     def _orthogonalize_batch(self, U, ns_steps):
@@ -336,11 +340,12 @@ class NorMuonGNS(torch.optim.Optimizer):
             return
         scales, step_ptrs, counts, _ = m8
         for table, states in counts:
-            for j, st in enumerate(states):
-                st["momentum_step"] += 1
-                table[j] = st["momentum_step"] & 0xFFFFFFFF
+            table[:] = [(st["momentum_step"] + 1) & 0xFFFFFFFF for st in states]
         _lib.check(lib.b2o_normuon_front8_multi(arr, scales, step_ptrs, n, dtc, beta, nesterov, gs, stream),
                    "normuon_front8")
+        for _, states in counts:  # a refused call leaves them
+            for st in states:
+                st["momentum_step"] += 1
         if x0:
             _lib.check(lib.b2o_normuon_prescale8(arr, scales, n, dtc, beta, nesterov, gs, self.norm_eps,
                                                  self.norm_safety, stream), "normuon_prescale8")
@@ -592,6 +597,10 @@ class NorMuonGNS(torch.optim.Optimizer):
                 loss = closure()
         hooked = self._hook_overridden()
         owned = self._owned
+        if self.momentum_dtype is not None:
+            for group in self.param_groups:  # before any group steps
+                if any(p.grad is not None for p in group["params"]):
+                    self._check_8bit_group(group)
         for gi, group in enumerate(self.param_groups):
             params = []
             for p in group["params"]:

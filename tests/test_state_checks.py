@@ -2,6 +2,7 @@
 pointers. Everything runs on the host: the launches are replaced, so that a state
 that slips through is seen in the descriptors and touches no memory."""
 import contextlib
+import ctypes
 import io
 
 import pytest
@@ -285,3 +286,75 @@ def test_loaded_types_become_those_that_the_kernels_read(host):
     adam.load_state_dict(sd)
     assert torch.equal(adam.state[q]["exp_avg"], x) and adam._steps[id(q)] == 3
     adam.step()
+
+
+# -------------------------------------------------------------- refused calls --
+@pytest.mark.parametrize("hooked", [False, True])
+def test_a_refused_front_call_leaves_the_step_counts(host, hooked):
+    """The count is the t of the codes: after a refusal a step has to be the one that it would have been."""
+    p, opt = _muon(momentum_dtype=torch.int8)
+    if hooked:
+        opt._orthogonalize_batch = lambda U, n: torch.zeros_like(U)
+    opt.step()
+    host.fail = "b2o_normuon_front8_multi"
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="front8"):
+            opt.step()
+    assert opt.state[p]["momentum_step"] == 1
+    host.fail = None
+    opt.step()
+    assert opt.state[p]["momentum_step"] == 2
+
+
+def test_the_counts_that_the_front_call_gets(host):
+    p, opt = _muon(momentum_dtype=torch.int8)
+    q = torch.nn.Parameter(torch.zeros(64, 128, dtype=torch.bfloat16))
+    q.grad = torch.ones_like(q)
+    opt.add_param_group({"params": [q]})
+    opt._init_state(q)["momentum_step"] = 2 ** 32 - 1
+    seen = []
+    real = host.__getattr__
+
+    def look(name):
+        call = real(name)
+        if name != "b2o_normuon_front8_multi":
+            return call
+        return lambda arr, scales, steps, n, *a: seen.append(
+            [ctypes.cast(steps[0], ctypes.POINTER(ctypes.c_uint32))[0]]) or call(arr, scales, steps, n, *a)
+    type(host).__getattr__, keep = lambda self, name: look(name), type(host).__getattr__
+    try:
+        opt.step()
+        opt.step()
+    finally:
+        type(host).__getattr__ = keep
+    assert seen == [[1], [0], [2], [1]] and opt.state[q]["momentum_step"] == 2 ** 32 + 1
+
+
+def test_momentum_out_of_range_is_refused_before_any_group_steps(host):
+    p, opt = _muon(momentum_dtype=torch.int8)
+    q = torch.nn.Parameter(torch.zeros(64, 128, dtype=torch.bfloat16))
+    q.grad = torch.ones_like(q)
+    opt.add_param_group({"params": [q]})
+    for bad in (1.0, -0.1, float("nan")):
+        opt.param_groups[1]["momentum"] = bad
+        with pytest.raises(ValueError, match="momentum in"):
+            opt.step()
+    assert host.calls == []
+    q.grad = None  # takes no part
+    opt.step()
+    wide = NorMuonGNS([torch.nn.Parameter(torch.zeros(4, 4))], momentum=1.0)
+    assert wide.param_groups[0]["momentum"] == 1.0
+
+
+@pytest.mark.parametrize("state_dtype,call", [(torch.int8, "b2o_adamw8_step"), (torch.float32, "b2o_adamw_step")])
+def test_a_refused_adamw_call_leaves_the_step_counts(host, state_dtype, call):
+    p, opt = _adamw(state_dtype=state_dtype)
+    opt.step()
+    host.fail = call
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="adamw"):
+            opt.step()
+    assert opt._steps[id(p)] == 1
+    host.fail = None
+    opt.step()
+    assert opt._steps[id(p)] == 2
