@@ -176,10 +176,11 @@ class NorMuonGNS(torch.optim.Optimizer):
         coeffs, resets, nres = self._table(ns_steps)
         mode = 0 if self.orthogonalizer == "quintic" else 1
         ortho = self._ortho_ws(U.device, ("single", S, r, c), ws["ortho_bytes"])
-        rc = lib.b2o_orthogonalize(U.data_ptr(), partial.data_ptr(), S, r, c, mode, coeffs, ns_steps, resets,
-                                   nres, self.norm_eps, self.norm_safety, ortho.data_ptr(),
-                                   ortho.numel(), out.data_ptr(), ws["rowsq"].data_ptr(),
-                                   _lib.stream_ptr(U.device))
+        with _lib.on_device(U.device):
+            rc = lib.b2o_orthogonalize(U.data_ptr(), partial.data_ptr(), S, r, c, mode, coeffs, ns_steps, resets,
+                                       nres, self.norm_eps, self.norm_safety, ortho.data_ptr(),
+                                       ortho.numel(), out.data_ptr(), ws["rowsq"].data_ptr(),
+                                       _lib.stream_ptr(U.device))
         _lib.check(rc, "orthogonalize")
 
     def load_state_dict(self, state_dict):
@@ -369,8 +370,9 @@ class NorMuonGNS(torch.optim.Optimizer):
                                            xscale=ws["xscale"].data_ptr(), flags=ws["flags"].data_ptr(),
                                            x0_half=int(b["x0"]))
             gs = self._grad_scale.data_ptr() if self._grad_scale is not None else None
-            self._front_call(lib, arr, len(members), _lib.dtype_code(dt), beta, int(bool(group["nesterov"])), gs, dev,
-                             any(b["x0"] for b in members), m8)
+            with _lib.on_device(dev):
+                self._front_call(lib, arr, len(members), _lib.dtype_code(dt), beta, int(bool(group["nesterov"])), gs,
+                                 dev, any(b["x0"] for b in members), m8)
 
     def _ortho_class(self, batches, ns_steps):
         """Orthogonalises every batch of one m = min(r, c) class with one library call."""
@@ -392,8 +394,9 @@ class NorMuonGNS(torch.optim.Optimizer):
             e0 = torch.cuda.Event(enable_timing=True)
             e0.record()
             n0 = _lib.launch_count()
-        rc = lib.b2o_orthogonalize_multi(groups, len(batches), mode, coeffs, ns_steps, resets, nres, self.norm_eps,
-                                         self.norm_safety, ortho.data_ptr(), ortho.numel(), _lib.stream_ptr(dev))
+        with _lib.on_device(dev):
+            rc = lib.b2o_orthogonalize_multi(groups, len(batches), mode, coeffs, ns_steps, resets, nres, self.norm_eps,
+                                             self.norm_safety, ortho.data_ptr(), ortho.numel(), _lib.stream_ptr(dev))
         _lib.check(rc, "orthogonalize_multi")
         if ev is not None:
             e1 = torch.cuda.Event(enable_timing=True)
@@ -432,9 +435,10 @@ class NorMuonGNS(torch.optim.Optimizer):
                                            o=b["o"].data_ptr(), rowsq=ws["rowsq"].data_ptr(),
                                            params=_lib.addr(pptr), rems=_lib.addr(rems), emas=_lib.addr(emas),
                                            vrows=_lib.addr(vrows), scratch=ws["scratch"].data_ptr())
-            rc = lib.b2o_normuon_apply_multi(arr, len(members), _lib.dtype_code(dt), -lr, lr * wd, 1.0 - lr * wd,
-                                             1 if wd else 0, int(bool(self.cautious_wd and wd)), 1.0 - beta2,
-                                             self._ema_weight, _lib.stream_ptr(dev))
+            with _lib.on_device(dev):
+                rc = lib.b2o_normuon_apply_multi(arr, len(members), _lib.dtype_code(dt), -lr, lr * wd, 1.0 - lr * wd,
+                                                 1 if wd else 0, int(bool(self.cautious_wd and wd)), 1.0 - beta2,
+                                                 self._ema_weight, _lib.stream_ptr(dev))
             _lib.check(rc, "normuon_apply")
 
     def _step_group(self, batches, group):

@@ -358,3 +358,34 @@ def test_a_refused_adamw_call_leaves_the_step_counts(host, state_dtype, call):
     host.fail = None
     opt.step()
     assert opt._steps[id(p)] == 2
+
+
+# ------------------------------------------------------------------ the device --
+@pytest.mark.parametrize("kw", [{}, dict(momentum_dtype=torch.int8)])
+@pytest.mark.parametrize("hooked", [False, True])
+def test_every_launch_of_a_muon_step_runs_on_its_parameters_device(host, monkeypatch, kw, hooked):
+    """With an overridden _orthogonalize_batch too, which calls the engine's own here."""
+    current = []
+
+    @contextlib.contextmanager
+    def on_device(dev):
+        current.append(dev)
+        yield
+        current.pop()
+    monkeypatch.setattr(_lib, "on_device", on_device)
+    p, opt = _muon(**kw)
+    if hooked:
+        inner = opt._orthogonalize_batch
+        opt._orthogonalize_batch = lambda U, n: inner(U, n)
+    real, where = host.__getattr__, []
+
+    def look(name):
+        call = real(name)
+        return call if call.__name__ != "call" else lambda *a: where.append((name, list(current))) or call(*a)
+    type(host).__getattr__, keep = lambda self, name: look(name), type(host).__getattr__
+    try:
+        opt.step()
+    finally:
+        type(host).__getattr__ = keep
+    assert any("front" in n for n, _ in where) and any("orthogonalize" in n for n, _ in where)
+    assert all(on == [p.device] for _, on in where), where
