@@ -197,7 +197,7 @@ class AdamW(torch.optim.Optimizer):
         pair = 2 | _lib.F32 << 32
         out, rows, last, extend = [], state8.Rows(), None, None
         empty, eight, f32, states = torch.empty_like, torch.int8, torch.float32, self.state
-        checked, unseen = self._checked, (None,) * 9
+        checked, unseen, mine = self._checked, (None,) * 9, None
         for p in params:
             index = p.get_device()
             if index != last:
@@ -205,6 +205,10 @@ class AdamW(torch.optim.Optimizer):
                 last, extend = index, rows.extend(index)
             st = states.get(p)
             if not st or "exp_avg" not in st:
+                if mine is None:
+                    mine = {id(q) for g in self.param_groups for q in g["params"]}
+                if id(p) not in mine:
+                    raise ValueError("AdamW.expanded_state: a parameter that is not this optimizer's")
                 st = self._init_state(p)
             m, v, n = st["exp_avg"], st["exp_avg_sq"], p.numel()
             get = st.get

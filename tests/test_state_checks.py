@@ -389,3 +389,14 @@ def test_every_launch_of_a_muon_step_runs_on_its_parameters_device(host, monkeyp
         type(host).__getattr__ = keep
     assert any("front" in n for n, _ in where) and any("orthogonalize" in n for n, _ in where)
     assert all(on == [p.device] for _, on in where), where
+
+
+def test_expanded_state_refuses_a_parameter_of_another_optimizer(host):
+    """It would get a state here, and state_dict() could no longer name its parameter."""
+    p, opt = _adamw()
+    q, _ = _adamw()
+    with pytest.raises(ValueError, match="not this optimizer"):
+        opt.expanded_state([p, q])
+    assert q not in opt.state and host.rows == []
+    assert set(opt.state_dict()["state"]) == {0}
+    opt.expanded_state([p, p])
