@@ -113,7 +113,9 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
   const BlockScale sv = root_scale(block_max<1>(&v));
   // Roots for the update and the codes. With a remainder the stored weight has
   // twice the bits, and the root gets a residual step (Newton: s + (v - s^2) /
-  // (2 s)); 0 and subnormal v keep a root near 0.
+  // (2 s)). Its remainder v - s^2 takes subnormal numbers as 0: 0 and subnormal v
+  // keep the root 0, which sends their codes to the exact path, and a v below
+  // 2^-103 keeps s, of which eps covers the last places.
   V8 r;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -123,7 +125,7 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
     else r.p[j] = f2(sqrt_approx(x.x), sqrt_approx(x.y));
     if (REM && EXTRA < 2) {
       const F2 inv = f2(fminf(rsqrt_approx_ftz(x.x), 9.2233720e18f), fminf(rsqrt_approx_ftz(x.y), 9.2233720e18f));
-      const F2 rest = fma2(mul2(r.p[j], f2(-1.0f)), r.p[j], v.p[j]);
+      const F2 rest = fma2_ftz(mul2(r.p[j], f2(-1.0f)), r.p[j], v.p[j]);
       r.p[j] = fma2(rest, mul2(inv, f2(0.5f)), r.p[j]);
     }
   }

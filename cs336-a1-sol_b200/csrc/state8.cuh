@@ -103,6 +103,12 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+// with subnormal operands and results taken as 0
+__device__ __forceinline__ F2 fma2_ftz(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 // a b + c with the product and the sum each rounded by itself. The sum is a
 // fused product one + c with one = 1 from the kernel's arguments: a packed
 // product and a packed sum are contracted into one rounding, although both say

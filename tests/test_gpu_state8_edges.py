@@ -159,3 +159,24 @@ def test_a_tensors_step_does_not_depend_on_what_shares_its_call(cuda, dtype, mas
     for k, (p, q, o) in enumerate(zip(mixed, alone, opts[1:])):
         assert torch.equal(p, q), k
         assert all(torch.equal(opts[0].state[p][x], o.state[q][x]) for x in o.state[q]), k
+
+
+@pytest.mark.parametrize("dtype,master", FORMS)
+@pytest.mark.parametrize("eps", [1e-8, 0.0])
+@pytest.mark.parametrize("size", [1e-22, 1e-20, 1e-19, 3e-19, 1e-18, 1e-15])
+def test_codes_of_second_moments_near_the_smallest_numbers(cuda, dtype, master, eps, size):
+    """Squares that are subnormal, 0 or just normal, in blocks of their own and beside each other: codes and scales are
+    the restatement's in every form (bf16 keeps such gradients, and a remainder changes how the roots are taken)."""
+    n = 8192 + 1000
+    p = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=cuda))
+    opt = _optimizer([p], master=master, eps=eps)
+    st = _state(n)
+    for step in range(1, 4):
+        g = _gen(int(-math.log10(size)) * 10 + step)
+        x = torch.randn(n, generator=g) * size * torch.where(torch.rand(n, generator=g) < 0.1, 30.0, 1.0)
+        x = x.to(dtype)
+        p.grad = x.cuda()
+        opt.step()
+        ref.adamw_step(torch.zeros(n, dtype=dtype), None, x, st, lr=0.0, betas=(0.9, 0.95), eps=1.0, wd=0.0, cautious=False, step=step)
+        for k in KEYS:
+            assert torch.equal(opt.state[p][k].cpu(), st[k]), (k, step)
