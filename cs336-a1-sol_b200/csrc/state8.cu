@@ -132,7 +132,7 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
   // A second moment that has overflowed (its block's scale is then NaN and its
   // codes 0): the quotient is m / inf, 0 for a finite m, but the residual steps
   // would make it inf * 0. Its root is set so that the denominator is finite and
-  // its reciprocal 0. One test for 8 elements costs nothing that shows (69.6 us
+  // its reciprocal 0. One test for 8 elements costs nothing that shows (69.7 us
   // for 33.5 M bf16 weights); a test at each pair's quotient took 72.8.
   if (EXTRA < 2 && isnan(sv.s)) {
 #pragma unroll
@@ -210,10 +210,12 @@ __device__ __forceinline__ void adamw8_tile(const b2o_adamw8_tensor& T, const Ad
 }
 
 // 256 threads, a chunk of 8192 elements a CTA, 3 or 4 CTAs an SM (80 or 64
-// registers). Measured on 33.5 M elements (a 32768 x 1024 table), against copy
-// bandwidth: bf16 weights 69 us (75 %, bound by instruction issue: 57 an
-// element), with a remainder 85 us (85 %), with the EMA too 121 us (94 %); fp32
-// 84 us (98 %), with the EMA 123 us (100 %). The residual steps of quotient and
+// registers). Measured on 33.5 M elements (a 32768 x 1024 table) without zeros,
+// against copy bandwidth: bf16 weights 70 us (74 %, bound by instruction issue: 58
+// an element), with weight decay 78 us (66 %; 65 instructions, no two-step unroll),
+// with a remainder 83 us (87 %), with a remainder and cautious decay 97 us (74 %; 82
+// instructions), with remainder and EMA 118 us (96 %); fp32 83 us (99 %), with decay
+// 88 us (94 %), with the EMA 123 us (100 %). The residual steps of quotient and
 // root cost 2 and 4 us where issue binds. Without the loads a step ahead the
 // first of these took 102 us; with 2 CTAs an SM 145; 16 elements a lane instead
 // of 8 took 19 % fewer instructions and the same time (fewer warps).
@@ -562,7 +564,9 @@ __device__ __forceinline__ void state_chunk(const b2o_state_tensor& T, int64_t b
 
 // 5 CTAs an SM (48 registers): the writing of codes is issue-bound and needs the
 // warps (33.5 M elements, signed: bf16 25.9 us against 30.8 with 3, fp32 26.7
-// against 31.5; with one tile a step instead of two 28.4 and 30.2).
+// against 31.5; with one tile a step instead of two 28.4 and 30.2). From bf16 it is
+// at 60 % (signed) and 53 % (root) of copy bandwidth with the ALU pipe 74 and 69 %
+// busy and issue slots 64 and 63 %: neither is full, so latency has a part.
 template <bool ENCODE>
 __global__ void __launch_bounds__(kS8Threads, 5) state_kernel(const __grid_constant__ StateTable tab) {
   pdl_wait();

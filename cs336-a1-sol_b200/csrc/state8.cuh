@@ -18,12 +18,19 @@
 // become zero would stay at 9 of 127 codes for good. In a step, u therefore
 // runs evenly over [0, 1): u = h / 2^32 to 23 bits, h = A i + B t (+ 2^31 for
 // signed) mod 2^32 for element i of the tensor and step t, A = 2^32 / golden
-// ratio, B = 2^32 (sqrt 2 - 1): turns that leave no wide gap. The rounding is
-// then right on average over steps, with no random state to keep. Simulated
-// updates (128-element blocks, lognormal scales of the elements with sigma 0.3,
-// betas 0.9 / 0.95, .99, .999) are off by 3.2, 3.5 and 3.8 % rms against 2.9, 6.3
-// and 5.4 % to nearest. A conversion (encode) uses u = 1/2, so that what was
-// decoded encodes to the same codes.
+// ratio, B = 2^32 (sqrt 2 - 1): turns that leave no wide gap. The code is then
+// right on average over steps, with no random state to keep. A conversion
+// (encode) uses u = 1/2, so that what was decoded encodes to the same codes.
+//
+// What it costs (oracle/state8_accuracy.py, betas 0.9 / 0.95, standard deviations
+// of a block's elements lognormal with sigma 0.3, 1.0, 1.5): updates are off by
+// 2.2, 6.5 and 21 % rms; to nearest by 2.0, 5.7 and 15 %, so in a steady run u is
+// a little worse. At beta2 = 0.999: 4.3, 9.9, 22 % against 3.6, 8.8, 20 %. Elements
+// whose gradient stops move on by 2.3 to 2.5 lr in 600 steps (64-bit moments: 2.3;
+// to nearest 12 to 22). The code is right on average, its value is not: that is
+// the code's square (second moments: fourth power), so second moments lie 1 to 2 %
+// high where their root is 0.003 to 0.03 of the block's largest, 13 % below that
+// (beta2 = 0.999: 4 to 6 %, 20 %).
 //
 // A code is exact: it depends on nothing but the fp32 state, its block's fp32
 // scale and u. The fast path computes y = levels sqrt(x / s) with approximate
@@ -38,7 +45,12 @@
 // bandwidth) at 103 instructions an element. Hence the fixed point, packed pairs
 // of floats (two roundings an instruction, each as the scalar one), the block
 // maximum in reduction instructions, one kernel for each set of options, and
-// the next step's loads ahead of this one's work: 69 us at 57 instructions.
+// the next step's loads ahead of this one's work: 70 us at 58 instructions.
+//
+// These times are for blocks without zeros. A second moment that is 0 or has sunk
+// to code 1 in a live block is settled one by one in 64 bits (size_codes): with 1,
+// 10 and 50 % of such elements, scattered, a bf16 step takes 83 to 89, 100 to 116
+// and 133 to 172 us, and an encode of second moments 44, 62 and 97 us against 29.
 //
 // Special blocks: a value that is not finite makes the scale NaN and every
 // code 0 (the whole block reads as NaN); s = 0 (for signed also s < 2^-126,
